@@ -1,0 +1,561 @@
+"""Losses of post-training on logits (``ops/losses.py``) against their definitions in float64 with autograd, on the CPU statements and on the kernels.
+
+Tolerances.  Of a row with soft-max p and target y, a kernel's gradient is c (onehot(y) - p), rounded once: half a step of its type.  Before that,
+relative to p: the exponent (z - m) log2 e is rounded to 32 bits (values of p above 2^-100: 100 * 2^-24 * ln 2 = 4.2e-6), ex2 is good to 2^-22,
+the sum of V terms in at most V / 512 + 16 steps to 2^-24 each on its way (256 steps: 1.5e-5 at V = 131072, far less as they are of both signs), lse in 32 bits to
+2^-24 * 32 = 2e-6; c follows lp with the same errors.  REL = 4e-5 holds them all.  lp itself: the sum's relative error, plus its own rounding."""
+import math
+
+import pytest
+import torch
+
+from transformers_fusion_b200.ops import _lib
+from transformers_fusion_b200.ops import losses as L
+
+REL = 4e-5
+TINY = 1e-30          # below it values may be flushed to zero (2^-100)
+IGN = -100
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def gen(device, seed=0):
+    return torch.Generator(device=device).manual_seed(seed)
+
+
+def make(device, lead, V, dtype, seed=0, ignored=0.3, idx=torch.int64):
+    g = gen("cpu", seed)
+    z = (3 * torch.randn(*lead, V, generator=g)).to(dtype)
+    y = torch.randint(0, V, lead, generator=g)
+    z.scatter_add_(-1, y[..., None], (8 * torch.rand(*lead, 1, generator=g)).to(dtype))
+    keep = torch.rand(lead, generator=g) >= ignored
+    return z.to(device), torch.where(keep, y, torch.full_like(y, IGN)).to(idx).to(device)
+
+
+def rows64(z, y):
+    """(kept rows, z in float64 with gradient, log p of the targets, zero on the others)."""
+    keep = y != IGN
+    z64 = torch.where(keep[..., None], z.double(), torch.zeros((), dtype=torch.float64, device=z.device)).requires_grad_(True)
+    lp = torch.log_softmax(z64, -1).gather(-1, y.long().clamp(min=0)[..., None])[..., 0]
+    return keep, z64, torch.where(keep, lp, torch.zeros((), dtype=torch.float64, device=z.device))
+
+
+def near(got, want, tol, what=""):
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    same = (got == want) | (got.isnan() & want.isnan())
+    bad = ~same & ~((got - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), (got - want).abs()[bad].max().item(), got[bad][:4].tolist(), want[bad][:4].tolist())
+
+
+def lp_tol(lp):
+    return REL / 2 + 2 ** -23 * lp.abs()
+
+
+def grad_tol(want, c, p, hot, dtype):
+    """Half a step of the type, and REL of what the gradient is the difference of."""
+    return half(dtype) * want.abs() * (1 + REL) + REL * c.abs()[..., None] * (p + hot) + TINY
+
+
+def check_grad(got, z, y, c, dtype):
+    """got against c (onehot(y) - p), c in float64 (0 on ignored rows)."""
+    keep = y != IGN
+    p = torch.softmax(torch.where(keep[..., None], z.double(), torch.zeros((), dtype=torch.float64, device=z.device)), -1)
+    hot = torch.zeros_like(p).scatter_(-1, y.long().clamp(min=0)[..., None], 1.0)
+    want = torch.where(keep[..., None], c[..., None] * (hot - p), torch.zeros_like(p))
+    near(got, want, torch.where(keep[..., None], grad_tol(want, c, p, hot, dtype), torch.zeros_like(p)), "dlogits")
+
+
+SHAPES = [((1,), 1), ((1,), 2), ((3,), 7), ((2, 3), 64), ((17,), 260), ((5,), 513), ((2, 4), 1000), ((3,), 4096), ((3,), 4097), ((2, 3), 16385), ((3,), 32000),
+          ((2,), 50257), ((2, 2), 65537), ((2,), 128256), ((2,), 131073), ((1,), 262149)]
+
+
+# ------------------------------------------------------------------------------------------------- log-probabilities
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lead,V", SHAPES)
+def test_logprobs(dev, dtype, lead, V):
+    z, y = make(dev, lead, V, dtype, V, idx=torch.int32 if V % 3 == 0 else torch.int64)
+    if len(lead) == 1 and lead[0] == 1:
+        y = y.clamp(min=0)
+    keep, z64, want = rows64(z, y)
+    lp, stats = L.logprobs_fwd(z, y)
+    assert lp.dtype == stats.dtype == F32
+    near(lp, want.detach(), lp_tol(want.detach()), "logp")
+    w_lse = torch.logsumexp(z64, -1).detach() * keep
+    near(stats.sum(0), w_lse, lp_tol(w_lse), "lse")
+    c = torch.randn(lead, generator=gen("cpu", 5)).to(dev)
+    check_grad(L.logprobs_bwd(c, z, y, stats), z, y, c.double(), dtype)
+    inside = z.clone().requires_grad_(True)                       # the autograd form
+    (g,) = torch.autograd.grad(L.token_logprobs(inside, y), inside, c)
+    assert torch.equal(g, L.logprobs_bwd(c, z, y, stats))
+    again = z.clone()                                             # in place
+    assert L.logprobs_bwd(c, again, y, stats, out=again) is again and torch.equal(again, g)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [33, 1000, 4099, 50257])
+@pytest.mark.parametrize("kind", ["no_last", "no_first", "sequence_major", "offset", "expanded", "out_offset", "padded"])
+def test_strides(dev, dtype, V, kind):
+    B, S = 3, 4
+    z, y = make(dev, (B, S + 1), V, dtype, V)
+    c, out = torch.randn(B, S, generator=gen("cpu", 5)).to(dev), None
+    if kind == "no_last":
+        z, y = z[:, :-1], y[:, 1:]
+    elif kind == "no_first":
+        z, y = z[:, 1:], y[:, :-1]
+    else:
+        y = y[:, 1:]
+        z0 = z[:, 1:].clone()
+        z = z0
+    if kind == "sequence_major":
+        z = z.transpose(0, 1).contiguous().transpose(0, 1)
+    elif kind == "offset":
+        z = torch.cat([z0.new_zeros(1), z0.flatten()])[1:].view(B, S, V)
+    elif kind == "expanded":
+        z = z[:, :1].expand(B, S, V)
+        out = torch.empty(B, S, V, dtype=dtype, device=dev)
+    elif kind == "out_offset":
+        out = torch.full((B * S * V + 3,), 7.0, dtype=dtype, device=dev)[3:].view(B, S, V)
+    elif kind == "padded":
+        z = torch.nn.functional.pad(z, (0, 5), value=float("nan"))[..., :V]
+        out = torch.full((B, S, V + 3), 7.0, dtype=dtype, device=dev)[..., :V]
+    keep, _, want = rows64(z, y)
+    lp, stats = L.logprobs_fwd(z, y)
+    near(lp, want.detach(), lp_tol(want.detach()))
+    g = L.logprobs_bwd(c, z, y, stats, out=out)
+    check_grad(g, z, y, c.double(), dtype)
+    if kind == "padded":                                          # behind the rows nothing is written
+        assert bool((out.as_strided((B, S, 3), (S * (V + 3), V + 3, 1), V) == 7).all())
+    A = torch.randn(B, S, generator=gen("cpu", 6)).to(dev)
+    o = L.policy_loss_fwd_bwd(z, y, A, clip=None, mean="sum", out=out)
+    check_grad(o.dlogits, z, y, -A.double(), dtype)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [40, 3000, 40000, 100001])
+def test_masked_values(dev, dtype, V):
+    """Rows: 0 a masked tail, 1 all but the target masked, 2 the target masked, 3 everything masked, 4 masks of the type's lowest value, 5 everything at it,
+    6 +inf, 7 NaN, 8 ignored with NaN and inf, 9 a target outside the vocabulary, 10 large values of both signs, 11 ordinary."""
+    g = gen("cpu", V)
+    z = (2 * torch.randn(12, V, generator=g)).to(dtype)
+    y = torch.randint(0, V // 2, (12,), generator=g)
+    low = torch.finfo(dtype).min
+    z[0, V // 2:] = -math.inf
+    z[1] = -math.inf
+    z[1, y[1]] = 1.5
+    z[2, y[2]] = -math.inf
+    z[3] = -math.inf
+    z[4, V // 2:] = low
+    z[5] = low
+    z[6, 3] = math.inf
+    z[7, V - 1] = math.nan
+    z[8, ::2], z[8, 1], y[8] = math.nan, math.inf, IGN
+    y[9] = V
+    z[10] *= 1e30
+    z, y = z.to(dev), y.to(dev)
+    c = torch.full((12,), 0.5, device=dev)
+    A = torch.full((12,), -0.5, device=dev)
+    lp, stats = L.logprobs_fwd(z, y)
+    d = L.logprobs_bwd(c, z, y, stats)
+    o = L.policy_loss_fwd_bwd(z, y, A, clip=None, mean="sum")
+    for name, got_lp, got in (("logprobs", lp, d), ("policy", o.logp, o.dlogits)):
+        for bad in (3, 6, 7, 9):
+            assert got_lp[bad].isnan() and got[bad].isnan().any(), (name, bad)
+        assert got_lp[8] == 0 and not got[8].any()
+        assert got_lp[2] == -math.inf and got_lp[1].abs() < 1e-6
+        for r in (0, 1, 2, 4, 5, 10, 11):
+            check_grad(got[r:r + 1], z[r:r + 1], y[r:r + 1], c[r:r + 1].double(), dtype)
+            want = torch.log_softmax(z[r].double(), -1)[y[r]]
+            near(got_lp[r], want, REL / 2 + 2 ** -22 * abs(want.item()) if math.isfinite(want.item()) else 0.0, (name, r))
+    assert o.loss.isnan()
+
+
+# ------------------------------------------------------------------------------------------------- policy
+def policy64(z, y, A, old, ref, clip, kl_coef, kl, mean, n_valid=None):
+    keep, z64, lp = rows64(z, y)
+    lp = lp.detach().requires_grad_(True)
+    A = A.double()
+    A = (A[:, None] if A.dim() < lp.dim() else A).expand(lp.shape)
+    if old is None and clip is None:
+        s = A * lp
+    else:
+        r = torch.exp(lp - (old.double() if old is not None else lp.detach()))
+        s = r * A
+        if clip is not None:
+            s = torch.minimum(s, r.clamp(1 - clip[0], 1 + clip[1]) * A)
+    k = torch.zeros_like(lp)
+    if ref is not None:
+        x = ref.double() - lp
+        k = torch.exp(x) - 1 - x if kl == "k3" else x
+    w = keep.double()
+    if mean == "tokens":
+        w = w / (n_valid if n_valid is not None else max(1, int(keep.sum())))
+    elif mean == "sequences":
+        w = w / (max(1, w.shape[0] if w.dim() == 2 else 1) * w.sum(-1, keepdim=True).clamp(min=1))
+    l = -s + kl_coef * k
+    loss = (w * l).sum()
+    (c,) = torch.autograd.grad(loss, lp)
+    slack = REL * (c.abs().sum() + (w * (s.abs() + kl_coef * k.abs())).sum()).item() + TINY
+    kslack = REL * (w * (1 + k.abs() + (ref.double() - lp).abs().expm1() if ref is not None else k)).sum().item() + TINY
+    return loss.detach(), (w * k).sum().detach(), lp.detach(), c, slack, kslack
+
+
+POLICY = [dict(), dict(clip=None), dict(old=True), dict(old=True, clip=None), dict(old=True, clip=(0.1, 0.3), mean="sequences"), dict(ref=True, kl_coef=0.1),
+          dict(old=True, ref=True, kl_coef=0.05, kl="k1", mean="sum"), dict(old=True, ref=True, kl_coef=0.3, mean="sequences", per_seq=True), dict(ref=True, clip=None, kl="k1"),
+          dict(old=True, n_valid=37.0), dict(old=True, clip=0.0)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lead,V", [((1, 1), 5), ((3, 9), 260), ((2, 5), 9001), ((2, 3), 32000), ((1, 2), 50257), ((2, 1), 140000)])
+@pytest.mark.parametrize("kw", POLICY, ids=lambda kw: "-".join(f"{k}={v}" for k, v in kw.items()) or "plain")
+def test_policy(dev, dtype, lead, V, kw):
+    kw = dict(kw)
+    z, y = make(dev, lead, V, dtype, 3 + V)
+    if lead[0] > 1:
+        y[0] = IGN                                                # a sequence without tokens
+    g = gen("cpu", 9)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dev)
+    _, _, lp = rows64(z, y)
+    lp = lp.detach()
+    A = rand(lead[0]) if kw.pop("per_seq", False) else rand(*lead)
+    clip = kw.get("clip", 0.2)
+    bounds = None if clip is None else clip if isinstance(clip, tuple) else (clip, clip)
+    old = ref = n_valid = None
+    if kw.pop("old", False):
+        d = 0.25 * rand(*lead)
+        for edge in [math.log1p(-bounds[0]), math.log1p(bounds[1])] if bounds else []:      # no ratio within 1e-3 of a border
+            d = torch.where((d - edge).abs() < 2e-3, torch.full_like(d, edge + 2e-3 * (1 if edge >= 0 else -1)), d)
+        old = (lp - d).float()
+    if kw.pop("ref", False):
+        ref = (lp + 0.4 * rand(*lead)).float()
+    if "n_valid" in kw:
+        n_valid = kw["n_valid"]
+        kw["n_valid"] = torch.tensor(n_valid, device=dev)
+    loss, k, lp, c, slack, kslack = policy64(z, y, A, old, ref, bounds, kw.get("kl_coef", 0.0), kw.get("kl", "k3"), kw.get("mean", "tokens"), n_valid)
+    o = L.policy_loss_fwd_bwd(z, y, A, old, ref, **kw)
+    near(o.loss, loss, slack, "loss")
+    near(o.kl, k, kslack, "kl")
+    near(o.logp, lp, lp_tol(lp) * (y != IGN), "logp")
+    check_grad(o.dlogits, z, y, c, dtype)
+    quiet = L.policy_loss_fwd_bwd(z, y, A, old, ref, want_grad=False, **kw)
+    assert quiet.dlogits is None and torch.equal(quiet.loss, o.loss) and torch.equal(quiet.logp, o.logp)
+    w = z.clone()
+    again = L.policy_loss_fwd_bwd(w, y, A, old, ref, out=w, **kw)     # in place, and bit for bit again
+    assert again.dlogits is w and torch.equal(w, o.dlogits) and torch.equal(again.loss, o.loss)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_policy_clip_share_and_flat(dev):
+    """Which tokens the clip takes is counted, and [T, V] logits are one sequence."""
+    z, y = make(dev, (40,), 50, F32, 4, ignored=0.25)
+    _, _, lp = rows64(z, y)
+    r = torch.linspace(0.5, 1.5, 40, dtype=torch.float64, device=dev) + 0.003
+    A = torch.where(torch.arange(40, device=dev) % 2 == 0, 1.0, -1.0)
+    o = L.policy_loss_fwd_bwd(z, y, A, (lp.detach() - r.log()).float(), clip=(0.2, 0.3))
+    keep = y != IGN
+    lost = keep & (((r > 1.3) & (A > 0)) | ((r < 0.8) & (A < 0)))
+    near(o.clipped, lost.double().sum() / keep.sum(), 1e-6)
+    assert not o.dlogits[lost | ~keep].any() and bool(o.dlogits[keep & ~lost].any(-1).all())
+    one = L.policy_loss_fwd_bwd(z[None], y[None], A[None], (lp.detach() - r.log()).float()[None], clip=(0.2, 0.3), mean="sequences")
+    assert torch.equal(one.dlogits[0], o.dlogits) and torch.equal(one.loss, o.loss)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("shape", [(2, 3), (0, 3), (2, 0), (0,)])
+def test_nothing_to_train_on(dev, shape):
+    z = torch.full((*shape, 11), math.nan, device=dev)
+    y = torch.full(shape, IGN, device=dev)
+    o = L.policy_loss_fwd_bwd(z, y, torch.full(shape, math.nan, device=dev), mean="tokens")
+    assert o.loss == 0 and o.kl == 0 and not o.dlogits.any() and o.dlogits.shape == z.shape
+    lp, stats = L.logprobs_fwd(z, y)
+    assert not lp.any() and not stats.any() and not L.logprobs_bwd(torch.ones(shape, device=dev), z, y, stats).any()
+    d = L.distill_loss_fwd_bwd(z, torch.full((*shape, 4), -1, device=dev), torch.zeros(*shape, 4, device=dev))
+    assert d.loss == 0 and not d.dlogits.any() and not d.kl.any()
+    if len(shape) == 2:
+        p = L.preference_loss_fwd_bwd(z, y, torch.arange(shape[0], device=dev).float())
+        want = torch.nn.functional.softplus(torch.tensor(-0.1)) if shape[0] else torch.tensor(0.0)      # h = (0 - 0) - (0 - 1)
+        near(p.loss.cpu(), want, 1e-6)
+        assert not p.dlogits.any() and not p.logp.any()
+
+
+# ------------------------------------------------------------------------------------------------- preferences
+def preference64(z, y, ref, beta, kind, eps, average):
+    keep, _, lp = rows64(z, y)
+    lp = lp.detach().requires_grad_(True)
+    n = keep.sum(1).clamp(min=1) if average else 1
+    s = lp.sum(1) / n
+    d = s - (ref.double() if ref is not None else 0)
+    h = d[:len(d) // 2] - d[len(d) // 2:]
+    if kind == "sigmoid":
+        l = -(1 - eps) * torch.nn.functional.logsigmoid(beta * h) - eps * torch.nn.functional.logsigmoid(-beta * h)
+    elif kind == "hinge":
+        l = torch.relu(1 - beta * h)
+    else:
+        l = (h - 1 / (2 * beta)) ** 2
+    (c,) = torch.autograd.grad(l.mean(), lp)
+    return l.mean().detach(), (beta * h).detach(), s.detach(), c, keep
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,S,V", [(1, 1, 9), (3, 17, 260), (2, 5, 32000), (1, 3, 50257), (40, 2, 33)])
+@pytest.mark.parametrize("kw", [dict(), dict(label_smoothing=0.1, beta=0.5), dict(kind="hinge", beta=0.02), dict(kind="squared", average=True, beta=1.0), dict(average=True)],
+                         ids=["sigmoid", "smooth", "hinge", "squared", "average"])
+def test_preference(dev, dtype, N, S, V, kw):
+    z, y = make(dev, (2 * N, S), V, dtype, N + V)
+    if N > 1:
+        y[1] = IGN                                                # an empty answer
+    ref = None if N == 40 else (rows64(z, y)[2].detach().sum(1) * 0.97).float()
+    beta = kw.get("beta", 0.1)
+    loss, x, s, c, keep = preference64(z, y, ref, beta, kw.get("kind", "sigmoid"), kw.get("label_smoothing", 0.0), kw.get("average", False))
+    o = L.preference_loss_fwd_bwd(z, y, ref, **kw)
+    per = REL / 2 * keep.sum(1).clamp(min=1)                      # of a sum of log-probabilities
+    near(o.logp, s, per + 2 ** -23 * s.abs(), "logp")
+    wide = beta * (per[:N] + per[N:])
+    near(o.margins, x, wide + 2 ** -23 * x.abs(), "margins")
+    steep = 1 if kw.get("kind") != "squared" else 2 * (x / beta - 0.5 / beta).abs().max().item() / beta + 1
+    near(o.loss, loss, steep * wide.max().item() + 1e-6 * loss.abs().item(), "loss")
+    # the coefficient moves with the margin: by at most beta/4 (sigmoid), 2 / beta... per unit of x, relative to c
+    move = {"sigmoid": 1.0, "hinge": 0.0, "squared": 2.0 / beta ** 2}[kw.get("kind", "sigmoid")] * wide.max().item() * beta / N
+    p = torch.softmax(torch.where(keep[..., None], z.double(), torch.zeros((), dtype=torch.float64, device=dev)), -1)
+    hot = torch.zeros_like(p).scatter_(-1, y.long().clamp(min=0)[..., None], 1.0)
+    want = c[..., None] * (hot - p) * keep[..., None]
+    near(o.dlogits, want, grad_tol(want, c, p, hot, dtype) + move * (p + hot), "dlogits")
+    assert not o.dlogits[~keep].any()
+    again = L.preference_loss_fwd_bwd(z, y, ref, out=z, **kw)     # in place
+    assert torch.equal(again.dlogits, o.dlogits) and again.dlogits is z and torch.equal(again.loss, o.loss)
+    assert L.preference_loss_fwd_bwd(o.dlogits, y, ref, want_grad=False, **kw).dlogits is None
+
+
+# ------------------------------------------------------------------------------------------------- distillation
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lead,V,K", [((1,), 1, 1), ((3,), 7, 9), ((2, 5), 260, 20), ((3,), 4098, 1), ((4,), 32000, 64), ((2,), 50257, 255), ((2, 2), 20000, 1024), ((2,), 150001, 7)])
+@pytest.mark.parametrize("tau,kind", [(1.0, "distinct"), (2.0, "twice"), (0.5, "holes")])
+def test_distill(dev, dtype, lead, V, K, tau, kind):
+    g = gen("cpu", V + K)
+    z = (3 * torch.randn(*lead, V, generator=g)).to(dtype)
+    top = (2 * torch.randn(*lead, K, generator=g)).to(BF if kind == "holes" else F32)
+    ids = torch.randint(0, V, (*lead, K), generator=g)                # ids may come more than once
+    if kind == "distinct" and K <= V:
+        ids = torch.rand(*lead, V, generator=g).argsort(-1)[..., :K]
+    elif kind == "twice" and K > 1:
+        ids[..., 1::2] = ids[..., :1]
+    elif kind == "holes":
+        ids[..., 1:][torch.rand(*lead, K - 1, generator=g) < 0.4] = -1
+        ids[0] = -1                                                   # a row (a sequence) that is not trained on
+    ids = ids.to(torch.int32 if kind == "twice" else torch.int64)
+    z, top, ids = z.to(dev), top.to(dev), ids.to(dev)
+    keep, have = ids[..., 0] >= 0, ids >= 0
+    z64 = z.double().requires_grad_(True)
+    t64 = torch.where(have, top.double() / tau, torch.full((), -math.inf, dtype=torch.float64, device=dev))
+    lq = torch.log_softmax(torch.where(keep[..., None], t64, torch.zeros((), dtype=torch.float64, device=dev)), -1)
+    q = torch.where(have, lq.exp(), torch.zeros_like(lq))
+    lp = torch.log_softmax(z64 / tau, -1).gather(-1, ids.long().clamp(min=0))
+    kl = torch.where(have & (q > 0), q * (lq - lp), torch.zeros_like(q)).sum(-1)
+    n = max(1, int(keep.sum()))
+    loss = tau ** 2 * kl.sum() / n
+    (want,) = torch.autograd.grad(loss, z64)
+    o = L.distill_loss_fwd_bwd(z, ids, top, temperature=tau)
+    ktol = REL * (1 + torch.where(have & (q > 0), q * (lq.abs() + lp.abs()), torch.zeros_like(q)).sum(-1)).detach()
+    near(o.kl, kl.detach(), ktol, "kl")
+    near(o.loss, loss.detach(), tau ** 2 * ktol.sum().item() / n + 1e-6 * loss.item(), "loss")
+    p, back = torch.softmax(z64.detach() / tau, -1) * keep[..., None], torch.zeros(*lead, V, dtype=torch.float64, device=dev)
+    back.scatter_add_(-1, ids.long().clamp(min=0), q.detach())
+    near(o.dlogits, want, half(dtype) * want.abs() * (1 + REL) + REL * tau / n * (p + back) + TINY, "dlogits")
+    assert not o.dlogits[~keep].any()
+    part = L.distill_loss_fwd_bwd(z, ids, top, temperature=tau, n_valid=torch.tensor([4.0 * n], device=dev), want_grad=False)
+    near(part.loss * 4, o.loss, 1e-6 * o.loss.abs().item())
+    again = L.distill_loss_fwd_bwd(z, ids, top, temperature=tau, out=z)
+    assert torch.equal(again.dlogits, o.dlogits) and torch.equal(again.loss, o.loss)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [50, 40001])
+def test_distill_masked(dev, V):
+    """Rows: 0 a teacher's token that the student has masked (KL is infinite, its gradient is not), 1 the student's mask elsewhere, 2 a teacher's mask, 3 all of it,
+    4 an id outside the vocabulary, 5 ordinary."""
+    g = gen("cpu", V)
+    z = torch.randn(6, V, generator=g)
+    ids = torch.randint(0, V // 2, (6, 3), generator=g) // 3 * 3 + torch.arange(3)
+    top = torch.randn(6, 3, generator=g)
+    z[0, ids[0, 1]] = -math.inf
+    z[1, V - 5:] = -math.inf
+    top[2, 1] = -math.inf
+    top[3] = -math.inf
+    ids[4, 2] = V
+    z, ids, top = z.to(dev), ids.to(dev), top.to(dev)
+    o = L.distill_loss_fwd_bwd(z, ids, top, n_valid=torch.ones(1, device=dev))
+    assert o.kl[0] == math.inf and o.kl[3].isnan() and o.kl[4].isnan() and o.loss.isnan()
+    assert o.dlogits[3].isnan().any() and o.dlogits[4].isnan().any()
+    q = torch.softmax(top.double(), -1)
+    for r in (0, 1, 2, 5):
+        want = torch.softmax(z[r].double(), -1)
+        tol = REL * want
+        want = want.index_add(0, ids[r], -q[r])
+        near(o.dlogits[r], want, half(F32) * want.abs() + tol.index_add(0, ids[r], REL * q[r]) + TINY)
+        kl = torch.where(q[r] > 0, q[r] * (q[r].log() - torch.log_softmax(z[r].double(), -1)[ids[r]]), torch.zeros((), dtype=torch.float64, device=dev)).sum()
+        near(o.kl[r], kl, REL * (1 + kl.abs().item()) if r else 0)
+
+
+# ------------------------------------------------------------------------------------------------- scoring
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("lead,H,V", [((1,), 8, 1), ((3, 5), 64, 260), ((2,), 72, 1001), ((1, 129), 128, 2000), ((300,), 64, 517), ((257,), 512, 4000), ((2, 200), 256, 32000), ((61,), 1024, 50257),
+                                       ((513,), 136, 777)])
+def test_linear_logprobs(dev, lead, H, V):
+    g = gen("cpu", V)
+    x = torch.randn(*lead, H, generator=g).to(BF).to(dev)
+    w = (torch.randn(V, H, generator=g) * 2 / math.sqrt(H)).to(BF).to(dev)
+    y = torch.randint(0, V, lead, generator=g)
+    y = torch.where(torch.rand(lead, generator=g) < 0.2, torch.full_like(y, IGN), y).to(dev)
+    keep = y != IGN
+    z = x.double() @ w.double().t()
+    # a product of H terms in 32 bits: H * 2^-24 of the sum of their sizes at worst, and the statistics' own error
+    size = (x.double().abs() @ w.double().abs().t()).max().item()
+    lse = torch.logsumexp(z, -1) * keep
+    lp = (z.gather(-1, y.clamp(min=0)[..., None])[..., 0] * keep - lse)
+    got, got_lse = L.linear_logprobs(x, w, y)
+    tol = REL / 2 + 2 * H * 2 ** -24 * size
+    near(got, lp, tol * keep)
+    near(got_lse, lse, tol * keep)
+    xs = torch.nn.functional.pad(x, (0, 3))[..., :H]                  # rows of another pitch
+    ws = torch.nn.functional.pad(w, (1, 0))[:, 1:]
+    near(L.linear_logprobs(xs, ws, y.int())[0], lp, tol * keep)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_linear_logprobs_special(dev):
+    """A target outside the vocabulary gives NaN, ignored rows of NaN and empty inputs give nothing."""
+    x, w = torch.randn(200, 64).to(BF).to(dev), torch.randn(300, 64).to(BF).to(dev)
+    y = torch.arange(200, device=dev)
+    y[5], y[6], y[7] = 300, -3, IGN
+    x[7] = math.nan
+    lp, lse = L.linear_logprobs(x, w, y)
+    assert lp[5].isnan() and lp[6].isnan() and lp[7] == 0 and lse[7] == 0
+    rest = torch.ones(200, dtype=torch.bool, device=dev)
+    rest[5:8] = False
+    assert lp[rest].isfinite().all() and lse[[5, 6]].isfinite().all()
+    assert L.linear_logprobs(x[:0], w, y[:0])[0].shape == (0,)
+    w[3] = math.inf * torch.ones(64, device=dev)
+    assert L.linear_logprobs(x[:5].abs(), w, y[:5])[0].isnan().all()
+
+
+# ------------------------------------------------------------------------------------------------- gradients by differences
+@pytest.mark.parametrize("dev", DEVICES)
+def test_gradients_by_differences(dev):
+    """Central differences of the loss along random directions.  h = 2^-5, |d| = 1 in every row: the third derivative of a row's loss is below 8 |c|
+    (h^2 / 6 * 8 = 1.3e-3 |c|), and a loss in 32 bits is off by 2^-23 of its terms (over 2 h: 2e-6)."""
+    B, S, V, h = 2, 4, 12, 2.0 ** -5
+    z, y = make(dev, (B, S), V, F32, 1, ignored=0.2)
+    g = gen("cpu", 2)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dev)
+    A, ref = rand(B, S), rows64(z, y)[2].detach().float() + 0.3 * rand(B, S)
+    ids = torch.rand(B, S, V, generator=g).argsort(-1)[..., :5].to(dev)
+    top = rand(B, S, 5)
+    kept = int((y != IGN).sum())
+    losses = [(lambda t: L.policy_loss_fwd_bwd(t, y, A, None, ref, clip=None, kl_coef=0.2), 3.0),
+              (lambda t: L.preference_loss_fwd_bwd(t, y, None, beta=0.5), 2.0 * kept),
+              (lambda t: L.distill_loss_fwd_bwd(t, ids, top, temperature=1.5), 1.5)]
+    for f, c in losses:
+        d = rand(B, S, V)
+        d = d / d.norm(dim=-1, keepdim=True)
+        o = f(z)
+        want = (f(z + h * d).loss - f(z - h * d).loss) / (2 * h)
+        near((o.dlogits.double() * d.double()).sum(), want.double(), 1.3e-3 * c + 2e-5 * (1 + o.loss.abs().item()))
+
+
+# ------------------------------------------------------------------------------------------------- refusals
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals(dev):
+    z, y = torch.zeros(2, 3, 8, device=dev), torch.zeros(2, 3, dtype=torch.int64, device=dev)
+    A, f = torch.zeros(2, 3, device=dev), torch.zeros(2, 3, device=dev)
+    st = torch.zeros(2, 2, 3, device=dev)
+    ids, top = torch.zeros(2, 3, 4, dtype=torch.int64, device=dev), torch.zeros(2, 3, 4, device=dev)
+    P, Q, D, W = L.policy_loss_fwd_bwd, L.preference_loss_fwd_bwd, L.distill_loss_fwd_bwd, L.linear_logprobs
+    x, w, yy = torch.zeros(6, 16, dtype=BF, device=dev), torch.zeros(8, 16, dtype=BF, device=dev), torch.zeros(6, dtype=torch.int64, device=dev)
+    bad = [
+        lambda: L.logprobs_fwd(z.half(), y), lambda: L.logprobs_fwd(z.double(), y), lambda: L.logprobs_fwd(z[0, 0], y[0, 0]), lambda: L.logprobs_fwd(z, y[:1]),
+        lambda: L.logprobs_fwd(z, y.float()), lambda: L.logprobs_fwd(z[..., ::2], y), lambda: L.logprobs_fwd(z[..., :0], y),
+        lambda: L.logprobs_fwd(z[None], y[None]), lambda: L.logprobs_bwd(f.double(), z, y, st), lambda: L.logprobs_bwd(f, z, y, f),
+        lambda: L.logprobs_bwd(f, z, y, st, out=torch.zeros(2, 3, 8, dtype=BF, device=dev)), lambda: L.logprobs_bwd(f, z, y, st, out=z[:, :1].expand(2, 3, 8)),
+        lambda: L.logprobs_bwd(f[:, :2], z[:, :2], y[:, :2], st[..., :2], out=z[:, 1:]), lambda: L.logprobs_bwd(f, z, y, st, out=torch.zeros(2, 3, 16, device=dev)[..., ::2]),
+        lambda: P(z, y, A[0]), lambda: P(z, y, A[:, :2]), lambda: P(z, y, A.double()), lambda: P(z, y, A, f[:1]), lambda: P(z, y, A, None, f[:1]),
+        lambda: P(z, y, A, kl="k2"), lambda: P(z, y, A, mean="rows"), lambda: P(z, y, A, clip=-0.1), lambda: P(z, y, A, kl_coef=0.1),
+        lambda: P(z, y, A, mean="sum", n_valid=torch.ones(1, device=dev)), lambda: P(z, y, A, n_valid=torch.ones(2, device=dev)), lambda: P(z, y, A, want_grad=False, out=z),
+        lambda: Q(z[0], y[0]), lambda: Q(z[:1], y[:1]), lambda: Q(z, y, f[0]), lambda: Q(z, y, beta=0.0), lambda: Q(z, y, kind="dpo"),
+        lambda: Q(z, y, label_smoothing=0.5), lambda: Q(z, y, kind="hinge", label_smoothing=0.1),
+        lambda: D(z, ids[0], top[0]), lambda: D(z, ids[..., :0], top[..., :0]), lambda: D(z, ids, top[..., :2]), lambda: D(z, ids.float(), top), lambda: D(z, ids, top.double()),
+        lambda: D(z, ids, top, temperature=0.0), lambda: D(z, ids, top, temperature=math.inf), lambda: D(z, ids.repeat(1, 1, 300), top.repeat(1, 1, 300)),
+        lambda: W(x, w[:, :8], yy), lambda: W(x, w.float(), yy), lambda: W(x, w, yy[:2]), lambda: W(x.requires_grad_(True), w, yy), lambda: W(x.detach(), w[:0], yy),
+    ]
+    if dev == "cuda":
+        bad += [lambda: L.logprobs_fwd(z, y.cpu()), lambda: P(z, y, A.cpu()), lambda: D(z, ids, top.cpu()), lambda: W(x.detach(), w.cpu(), yy),
+                lambda: W(x.detach().float(), w.float(), yy), lambda: W(x.detach()[:, :9], w[:, :9], yy)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError(f"call {i} was taken")
+
+
+# ------------------------------------------------------------------------------------------------- GPU: streams, graphs, far rows
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    """Two captured graphs replayed on two streams at once, beside eager calls, give what one call alone gives."""
+    z, y = make("cuda", (4, 50), 32000, BF, 3)
+    A, old = torch.randn(4, 50, device="cuda"), torch.randn(4, 50, device="cuda") - 8
+    ids, top = torch.randint(0, 32000, (4, 50, 20), device="cuda"), torch.randn(4, 50, 20, device="cuda")
+    x, w = torch.randn(200, 256, device="cuda").to(BF), (torch.randn(32000, 256, device="cuda") / 16).to(BF)
+
+    def everything():
+        p = L.policy_loss_fwd_bwd(z, y, A, old, old, kl_coef=0.1)
+        q = L.preference_loss_fwd_bwd(z, y)
+        d = L.distill_loss_fwd_bwd(z, ids, top)
+        s = L.linear_logprobs(x, w, y.view(-1))
+        return [p.loss, p.kl, p.clipped, p.logp, p.dlogits, q.loss, q.margins, q.logp, q.dlogits, d.loss, d.kl, d.dlogits, *s]
+    want = [t.clone() for t in everything()]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    for s in streams:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            everything()
+            s.synchronize()
+            with torch.cuda.graph(graph, stream=s):
+                out = everything()
+        graphs.append((graph, out))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = everything()
+    torch.cuda.synchronize()
+    for got in (eager, graphs[0][1], graphs[1][1]):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    _lib.check_status()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows behind 2^31 values of bfloat16 logits, in place."""
+    V, T = 128256, 16800
+    z = torch.empty(T, V, dtype=BF, device="cuda").normal_(generator=gen("cuda", 1))
+    y = torch.full((T,), IGN, device="cuda")
+    y[::700] = torch.arange(24, device="cuda") * 5000
+    y[-1] = V - 1
+    rows = (y != IGN).nonzero()[:, 0]
+    keep, A = z[rows].clone(), torch.randn(T, device="cuda")
+    o = L.policy_loss_fwd_bwd(z, y, A, clip=None, mean="sum", out=z)
+    check_grad(z[rows], keep, y[rows], -A[rows].double(), BF)
+    near(o.logp[rows], torch.log_softmax(keep.double(), -1).gather(1, y[rows, None])[:, 0], 1e-4)
+    assert not z[1:700].any() and not z[-5:-1].any()

@@ -1,0 +1,479 @@
+"""Losses of post-training on logits, and the scoring of given tokens.
+
+* ``logprobs_fwd`` / ``logprobs_bwd``: log-probabilities of given tokens and the gradient of the logits; ``token_logprobs`` is both as one
+  autograd function.
+* ``policy_loss_fwd_bwd``: clipped policy loss with a KL term.
+* ``preference_loss_fwd_bwd``: loss of paired answers on their log-ratios to a reference model.
+* ``distill_loss_fwd_bwd``: KL divergence from a teacher's stored top logits.
+* ``linear_logprobs``: log-probabilities of given tokens from hidden states and the head's weight, for passes that want no gradient.
+
+As in ``ops/functional.py``: CUDA tensors go to the sm_100a kernels (``csrc/kernels/token_losses.cu``), CPU tensors run the plain PyTorch
+statement of the same mathematics.
+
+Logits are [T, V] or [B, S, V], bfloat16 or float32, of any strides with a dense last dimension (rows may start at any element).  Targets are
+int64 or int32 of the logits' leading shape; rows whose target is ``ignore_index`` are not read, their statistics and gradients are 0.  A
+target outside the vocabulary makes its row's results NaN.  ``out`` takes the gradient: another tensor of the logits' shape and type, or the
+logits themselves, which are then overwritten; None makes a new one.  Per-row results and losses are float32.
+
+Reference counterparts: log-probabilities, ratio clipping and KL terms of the RL trainers (src/trainer/trainer_rl.cpp:557-1350)."""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib, functional as F
+from ._lib import c_f, c_i, c_ll, c_p, check, ptr, stream
+
+MAX_TOP = 1024          # entries of a teacher's row
+
+_KL = {"k3": 0, "k1": 1}
+_MEAN = {"tokens": 0, "sequences": 1, "sum": 2}
+_KIND = {"sigmoid": 0, "hinge": 1, "squared": 2}
+
+
+class _Rows(C.Structure):
+    _fields_ = [("z", c_p), ("dz", c_p), ("zb", c_ll), ("zs", c_ll), ("db", c_ll), ("ds", c_ll), ("T", c_i), ("S", c_i), ("V", c_i), ("f32", c_i)]
+
+
+class _Policy(C.Structure):
+    _fields_ = [("targets", c_p), ("idx64", c_i), ("ignore", c_ll), ("adv", c_p), ("old_lp", c_p), ("ref_lp", c_p), ("adv_seq", c_i), ("ratio", c_i),
+                ("kl_kind", c_i), ("mean", c_i), ("lo", c_f), ("hi", c_f), ("kl_coef", c_f), ("n_valid", c_p), ("logp", c_p), ("out", c_p),
+                ("denom", c_p), ("terms", c_p)]
+
+
+class _Preference(C.Structure):
+    _fields_ = [("targets", c_p), ("idx64", c_i), ("ignore", c_ll), ("ref", c_p), ("kind", c_i), ("average", c_i), ("beta", c_f), ("smooth", c_f),
+                ("loss", c_p), ("margins", c_p), ("logp", c_p), ("lp64", c_p), ("stats", c_p), ("coef", c_p), ("terms", c_p)]
+
+
+class _Distill(C.Structure):
+    _fields_ = [("top_ids", c_p), ("top_z", c_p), ("idx64", c_i), ("top_f32", c_i), ("K", c_i), ("tau", c_f), ("n_valid", c_p), ("kl", c_p), ("loss", c_p),
+                ("denom", c_p), ("terms", c_p)]
+
+
+_lib.register("tfb_token_logprobs", [C.POINTER(_Rows), c_p, c_i, c_ll, c_p, c_p, c_p, c_p])
+_lib.register("tfb_token_logprobs_bwd", [C.POINTER(_Rows), c_p, c_i, c_ll, c_p, c_p, c_p])
+_lib.register("tfb_policy_loss", [C.POINTER(_Rows), C.POINTER(_Policy), c_p])
+_lib.register("tfb_preference_loss", [C.POINTER(_Rows), C.POINTER(_Preference), c_p])
+_lib.register("tfb_distill_loss", [C.POINTER(_Rows), C.POINTER(_Distill), c_p])
+
+
+# ---------------------------------------------------------------------------------------------
+# arguments
+# ---------------------------------------------------------------------------------------------
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _check_logits(logits, name="logits"):
+    _need(logits.dim() in (2, 3), f"{name}: [T, V] or [B, S, V], got {tuple(logits.shape)}")
+    _need(logits.dtype in (torch.bfloat16, torch.float32), f"{name}: bfloat16 or float32, got {logits.dtype}")
+    _need(logits.shape[-1] > 0, f"{name}: an empty vocabulary")
+    _need(logits.stride(-1) == 1 or logits.shape[-1] == 1, f"{name}: the last dimension has to be dense")
+
+
+def _check_index(idx, shape, name, device):
+    _need(idx.dtype in (torch.int64, torch.int32), f"{name}: int64 or int32, got {idx.dtype}")
+    _need(tuple(idx.shape) == tuple(shape), f"{name}: {tuple(shape)} wanted, got {tuple(idx.shape)}")
+    _need(idx.device == device, f"{name}: on {idx.device}, the logits are on {device}")
+    return idx.contiguous()
+
+
+def _check_f32(t, shape, name, device):
+    """A float32 tensor of this shape, dense; None stays None."""
+    if t is None:
+        return None
+    _need(t.dtype == torch.float32, f"{name}: float32, got {t.dtype}")
+    _need(tuple(t.shape) == tuple(shape), f"{name}: {tuple(shape)} wanted, got {tuple(t.shape)}")
+    _need(t.device == device, f"{name}: on {t.device}, the logits are on {device}")
+    return t.contiguous()
+
+
+def _check_n_valid(n_valid, device):
+    if n_valid is None:
+        return None
+    _need(n_valid.numel() == 1, "n_valid: one value")
+    return _check_f32(n_valid.reshape(1), (1,), "n_valid", device)
+
+
+def _gradient(logits, out, want_grad):
+    """Where the gradient goes: None, ``out``, or a new tensor."""
+    if not want_grad:
+        _need(out is None, "out: without want_grad there is no gradient")
+        return None
+    if out is None:
+        # rows of the same alignment as those of the logits where they are dense
+        return torch.empty_like(logits, memory_format=torch.preserve_format)
+    _need(out.shape == logits.shape and out.dtype == logits.dtype and out.device == logits.device, "out: the logits' shape, type and device")
+    _need(out.stride(-1) == 1 or out.shape[-1] == 1, "out: the last dimension has to be dense")
+    V, dims = out.shape[-1], sorted((out.stride(i), out.shape[i]) for i in range(out.dim() - 1) if out.shape[i] > 1)
+    reach = V
+    for stride, n in dims:
+        _need(stride >= reach, "out: its rows overlap")
+        reach = stride * (n - 1) + reach
+    if out.numel() and not (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()):
+        first, last = _span(out)
+        a, b = _span(logits)
+        _need(last <= a or b <= first, "out: overlaps the logits without being them")
+    return out
+
+
+def _span(t):
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))
+
+
+def _rows(logits, grad=None):
+    two = logits.dim() == 2
+    S = logits.shape[0] if two else logits.shape[1]
+    T = logits.shape[:-1].numel()
+    strides = lambda t: (0, 0) if t is None else ((0, t.stride(0)) if two else (t.stride(0), t.stride(1)))
+    zb, zs = strides(logits)
+    db, ds = strides(grad)
+    return _Rows(logits.data_ptr(), ptr(grad), zb, zs, db, ds, T, max(S, 1), logits.shape[-1], int(logits.dtype == torch.float32))
+
+
+def _on(device):
+    """The device of the tensors, current for the launch: streams and kernels belong to the device that is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _empty(device, *sizes, dtype=torch.float32):
+    return torch.empty(sizes, dtype=dtype, device=device)
+
+
+def _zero_(grad):
+    return grad.zero_() if grad is not None else None
+
+
+def _softmax64(z):
+    """CPU statement: (z - m, m, log of the sum of exp(z - m)) in float64, m the maximum of a row: apart, since m + log S is m where m is large."""
+    z = z.double()
+    m = z.max(-1).values
+    d = z - torch.where(m == -math.inf, torch.zeros_like(m), m)[..., None]
+    return d, m, torch.exp(d).sum(-1).log()
+
+
+def _taken(z, targets, ignore_index):
+    """CPU statement: (kept rows, target clamped into the vocabulary, log p of the target, 0 on the other rows, what ``_softmax64`` gives)."""
+    keep = targets != ignore_index
+    y = targets.long()
+    inside = (y >= 0) & (y < z.shape[-1])
+    y = y.clamp(0, z.shape[-1] - 1)
+    d, m, ls = _softmax64(z)
+    lp = d.gather(-1, y[..., None])[..., 0] - ls
+    lp = torch.where(inside, lp, torch.full_like(lp, math.nan))
+    return keep, y, torch.where(keep, lp, torch.zeros((), dtype=torch.float64)), (d, m, ls)
+
+
+def _row_gradient(y, c, soft, keep, grad):
+    """CPU statement: grad = c (onehot(y) - softmax z) on the kept rows."""
+    g = -torch.exp(soft[0] - soft[2][..., None])
+    g.scatter_add_(-1, y[..., None], torch.ones_like(g[..., :1]))
+    grad.copy_(torch.where(keep[..., None], g * c[..., None], torch.zeros((), dtype=g.dtype)).to(grad.dtype))
+
+
+# ---------------------------------------------------------------------------------------------
+# log-probabilities of given tokens
+# ---------------------------------------------------------------------------------------------
+def logprobs_fwd(logits, targets, ignore_index: int = -100):
+    """(log softmax(logits)[target], stats), float32: the first of the targets' shape, ``stats`` [2, *shape] the maximum m of every row and the log of its
+    sum of exp(z - m), whose sum is logsumexp(z); all 0 on ignored rows."""
+    _check_logits(logits)
+    targets = _check_index(targets, logits.shape[:-1], "targets", logits.device)
+    if not logits.is_cuda:
+        keep, _, lp, (_, m, ls) = _taken(logits, targets, ignore_index)
+        return lp.float(), torch.where(keep, torch.stack([m, ls]), torch.zeros((), dtype=m.dtype)).float()
+    lp, stats = _empty(logits.device, *targets.shape), _empty(logits.device, 2, *targets.shape)
+    _score_rows(logits, targets, ignore_index, lp, None, stats)
+    return lp, stats
+
+
+def _score_rows(logits, targets, ignore_index, lp, lse, stats):
+    if targets.numel():
+        with _on(logits.device):
+            check(_lib.lib().tfb_token_logprobs(_rows(logits), targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), ptr(lp), ptr(lse),
+                                                ptr(stats), stream()), "token_logprobs")
+
+
+def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=None):
+    """d logits = dlogp (onehot(target) - softmax(logits)); ``stats`` as ``logprobs_fwd`` gave them."""
+    _check_logits(logits)
+    targets = _check_index(targets, logits.shape[:-1], "targets", logits.device)
+    dlogp = _check_f32(dlogp, targets.shape, "dlogp", logits.device)
+    stats = _check_f32(stats, (2, *targets.shape), "stats", logits.device)
+    grad = _gradient(logits, out, True)
+    if not logits.is_cuda:
+        keep, y, lp, soft = _taken(logits, targets, ignore_index)
+        c = torch.where(lp.isnan(), lp, dlogp.double())
+        _row_gradient(y, c, soft, keep, grad)
+        return grad
+    if targets.numel():
+        with _on(logits.device):
+            check(_lib.lib().tfb_token_logprobs_bwd(_rows(logits, grad), targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index),
+                                                    stats.data_ptr(), dlogp.data_ptr(), stream()), "token_logprobs_bwd")
+    return grad
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, ignore_index):
+        lp, stats = logprobs_fwd(logits, targets, ignore_index)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.ignore_index = ignore_index
+        return lp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp):
+        logits, targets, stats = ctx.saved_tensors
+        return logprobs_bwd(dlogp.float(), logits, targets, stats, ctx.ignore_index), None, None
+
+
+def token_logprobs(logits, targets, ignore_index: int = -100):
+    """Log-probabilities of given tokens, float32 of the targets' shape, with the gradient of the logits."""
+    return _TokenLogprobs.apply(logits, targets, ignore_index)
+
+
+# ---------------------------------------------------------------------------------------------
+# policy
+# ---------------------------------------------------------------------------------------------
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor                     # scalar
+    kl: torch.Tensor                       # scalar: mean of the KL estimate (0 without reference log-probabilities)
+    clipped: torch.Tensor                  # scalar: share of the tokens whose gradient the clip took
+    logp: torch.Tensor                     # log-probabilities of the tokens
+    dlogits: Optional[torch.Tensor]
+
+
+def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logprobs=None, *, clip=0.2, kl_coef: float = 0.0, kl: str = "k3",
+                        mean: str = "tokens", n_valid=None, ignore_index: int = -100, want_grad: bool = True, out=None) -> PolicyLoss:
+    """Policy loss of sampled tokens and its gradient with respect to the logits, in one pass over them.
+
+    Per token, with lp its log-probability, A its advantage, r = exp(lp - old): -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef * KL.  ``clip`` is
+    one bound for both sides, (lo, hi), or None: no clip.  Without ``old_logprobs`` the tokens are the policy's own: r is 1 and its gradient that
+    of lp; without a clip as well the objective is A lp itself.  KL against ``ref_logprobs``, x = ref - lp: "k3" exp(x) - 1 - x (estimates KL(policy || reference)
+    on the policy's tokens), "k1" x (KL(reference || policy) on the reference's).
+
+    ``advantages``: one per token, or [B], one per sequence.  ``mean``: over all "tokens" (``n_valid``, one float32 value on the device, replaces their
+    number, for a batch in several calls), over the "sequences" of each one's mean over its tokens (a sequence without tokens counts as 0), or "sum"."""
+    _check_logits(logits)
+    dev = logits.device
+    targets = _check_index(targets, logits.shape[:-1], "targets", dev)
+    _need(kl in _KL, f"kl: one of {sorted(_KL)}, got {kl!r}")
+    _need(mean in _MEAN, f"mean: one of {sorted(_MEAN)}, got {mean!r}")
+    _need(mean == "tokens" or n_valid is None, "n_valid: belongs to the mean over tokens")
+    _need(kl_coef == 0.0 or ref_logprobs is not None, "kl_coef: wants reference log-probabilities")
+    adv_seq = logits.dim() == 3 and advantages.dim() == 1
+    advantages = _check_f32(advantages, targets.shape[:1] if adv_seq else targets.shape, "advantages", dev)
+    old, ref = _check_f32(old_logprobs, targets.shape, "old_logprobs", dev), _check_f32(ref_logprobs, targets.shape, "ref_logprobs", dev)
+    n_valid = _check_n_valid(n_valid, dev)
+    lo, hi = (math.inf, math.inf) if clip is None else (float(clip[0]), float(clip[1])) if isinstance(clip, (tuple, list)) else (float(clip), float(clip))
+    _need(lo >= 0 and hi >= 0, f"clip: bounds of 0 or more, got {clip!r}")
+    ratio = old is not None or clip is not None
+    grad = _gradient(logits, out, want_grad)
+    B, S = targets.shape if targets.dim() == 2 else (1, targets.shape[0])
+    if not logits.is_cuda:
+        keep, y, lp, soft = _taken(logits, targets, ignore_index)
+        zero = torch.zeros((), dtype=torch.float64)
+        A = (advantages[:, None] if adv_seq else advantages).double().expand(lp.shape)
+        clipped = torch.zeros_like(lp)
+        if ratio:
+            r = torch.exp(lp - old.double()) if old is not None else torch.exp(lp - lp)
+            s = ds = r * A
+            c = r.clamp(1 - lo, 1 + hi) * A
+            clipped = (c < s).double()
+            s, ds = torch.where(c < s, c, s), torch.where(c < s, zero, ds)
+        else:
+            s, ds = A * lp, A
+        k, dk = torch.zeros_like(lp), torch.zeros_like(lp)
+        if ref is not None:
+            x = ref.double() - lp
+            k, dk = (torch.expm1(x) - x, -torch.expm1(x)) if kl == "k3" else (x, -torch.ones_like(x))
+        w = keep.double()
+        if mean == "tokens":
+            w = w / (n_valid.double() if n_valid is not None else w.sum().clamp(min=1))
+        elif mean == "sequences":
+            w = w.view(B, S)
+            w = (w / (max(B, 1) * w.sum(1, keepdim=True).clamp(min=1))).view(keep.shape)
+        total = lambda v: torch.where(keep, w * v, zero).sum().float()
+        if grad is not None:
+            _row_gradient(y, torch.where(lp.isnan(), lp, w * (kl_coef * dk - ds)), soft, keep, grad)
+        return PolicyLoss(total(kl_coef * k - s), total(k), total(clipped), lp.float(), grad)
+    lp = _empty(dev, *targets.shape)
+    if not lp.numel():
+        z = torch.zeros((), device=dev)
+        return PolicyLoss(z, z, z, lp, grad)
+    sums, work = _empty(dev, 3), _empty(dev, 3 * lp.numel() + max(1, B))
+    arg = _Policy(targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), advantages.data_ptr(), ptr(old), ptr(ref), int(adv_seq), int(ratio),
+                  _KL[kl], _MEAN[mean], 1 - lo, 1 + hi, float(kl_coef), ptr(n_valid), lp.data_ptr(), sums.data_ptr(),
+                  work.data_ptr() + 12 * lp.numel(), work.data_ptr())
+    with _on(dev):
+        check(_lib.lib().tfb_policy_loss(_rows(logits, grad), arg, stream()), "policy_loss", 3)
+    return PolicyLoss(sums[0], sums[1], sums[2], lp, grad)
+
+
+# ---------------------------------------------------------------------------------------------
+# preferences
+# ---------------------------------------------------------------------------------------------
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor                     # scalar: mean over the pairs
+    margins: torch.Tensor                  # [N] beta times the difference of the log-ratios: > 0 where the chosen answer is preferred
+    logp: torch.Tensor                     # [2N] log-probabilities of the answers (their means with ``average``)
+    dlogits: Optional[torch.Tensor]
+
+
+def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float = 0.1, kind: str = "sigmoid", label_smoothing: float = 0.0,
+                            average: bool = False, ignore_index: int = -100, want_grad: bool = True, out=None) -> PreferenceLoss:
+    """Loss of N pairs of answers and its gradient: logits [2N, S, V] and targets [2N, S] hold the N chosen answers first, then the N rejected
+    ones, each padded with ``ignore_index``.
+
+    L_i is the sum of the log-probabilities of answer i (``average``: their mean), ``ref_logprobs`` [2N] the same under the reference model (None: 0), h
+    the difference (L - ref) of the chosen answer less that of the rejected one.  ``kind``: "sigmoid" -(1 - e) log sigmoid(beta h) - e log sigmoid(-beta h)
+    with e = ``label_smoothing``, "hinge" max(0, 1 - beta h), "squared" (h - 1 / (2 beta))^2."""
+    _check_logits(logits)
+    dev = logits.device
+    _need(logits.dim() == 3 and logits.shape[0] % 2 == 0, f"logits: [2N, S, V], got {tuple(logits.shape)}")
+    targets = _check_index(targets, logits.shape[:-1], "targets", dev)
+    _need(kind in _KIND, f"kind: one of {sorted(_KIND)}, got {kind!r}")
+    _need(beta > 0, f"beta: more than 0, got {beta}")
+    _need(0 <= label_smoothing < 0.5, f"label_smoothing: in [0, 0.5), got {label_smoothing}")
+    _need(label_smoothing == 0 or kind == "sigmoid", "label_smoothing: belongs to the sigmoid loss")
+    N, S = logits.shape[0] // 2, logits.shape[1]
+    ref = _check_f32(ref_logprobs, (2 * N,), "ref_logprobs", dev)
+    grad = _gradient(logits, out, want_grad)
+    if not logits.is_cuda:
+        keep, y, lp, soft = _taken(logits, targets, ignore_index)
+        n = keep.sum(1).clamp(min=1).double() if average else torch.ones(2 * N, dtype=torch.float64)
+        L = lp.sum(1) / n
+        d = L - (ref.double() if ref is not None else 0)
+        h = d[:N] - d[N:]
+        x = beta * h
+        if kind == "sigmoid":
+            l = torch.log1p(torch.exp(-x.abs())) + (-x).clamp(min=0) + label_smoothing * x
+            dl = beta * (label_smoothing - torch.sigmoid(-x))
+        elif kind == "hinge":
+            l, dl = (1 - x).clamp(min=0), torch.where(x.isnan(), x, -beta * (x < 1).double())
+        else:
+            l, dl = (h - 0.5 / beta) ** 2, 2 * (h - 0.5 / beta)
+        if grad is not None:
+            c = torch.cat([dl, -dl]) / max(N, 1) / n
+            _row_gradient(y, c[:, None].expand(lp.shape), soft, keep, grad)
+        return PreferenceLoss((l.sum() / max(N, 1)).float(), x.float(), L.float(), grad)
+    margins, L = _empty(dev, N), _empty(dev, 2 * N)
+    if N == 0 or S == 0:
+        # no pairs, or only empty answers: nothing depends on the logits
+        L.zero_()
+        d = L if ref is None else -ref
+        x = beta * (d[:N] - d[N:])
+        l = {"sigmoid": torch.nn.functional.softplus(-x) + label_smoothing * x, "hinge": (1 - x).clamp(min=0), "squared": (x / beta - 0.5 / beta) ** 2}[kind]
+        return PreferenceLoss(l.sum() / max(N, 1), x, L, grad)
+    T = 2 * N * S
+    loss, lp64, work = _empty(dev, 1), _empty(dev, T, dtype=torch.float64), _empty(dev, 2 * T + 3 * N)
+    arg = _Preference(targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), ptr(ref), _KIND[kind], int(average), float(beta),
+                      float(label_smoothing), loss.data_ptr(), margins.data_ptr(), L.data_ptr(), lp64.data_ptr(), work.data_ptr(),
+                      work.data_ptr() + 8 * T, work.data_ptr() + 8 * T + 8 * N)
+    with _on(dev):
+        check(_lib.lib().tfb_preference_loss(_rows(logits, grad), arg, stream()), "preference_loss", 4 if want_grad else 3)
+    return PreferenceLoss(loss[0], margins, L, grad)
+
+
+# ---------------------------------------------------------------------------------------------
+# distillation
+# ---------------------------------------------------------------------------------------------
+class DistillLoss(NamedTuple):
+    loss: torch.Tensor                     # scalar: temperature^2 times the mean of kl over the rows with entries
+    kl: torch.Tensor                       # per row, at the temperature
+    dlogits: Optional[torch.Tensor]
+
+
+def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.0, n_valid=None, want_grad: bool = True, out=None) -> DistillLoss:
+    """Distillation from the top logits of a teacher, and its gradient, in one pass over the student's logits.
+
+    ``top_ids`` (int64 or int32) and ``top_logits`` (bfloat16 or float32) are the logits' leading shape + [K], K up to 1024: the teacher's best
+    tokens of every row with their logits (or log-probabilities: only differences count).  Negative ids are entries that are not there; a row
+    whose first id is negative has none and is not trained on.  With q the soft-max of a row's entries at the temperature and p that of the
+    student's whole row, KL = sum q (log q - log p); loss = temperature^2 mean KL.  An id that comes twice counts twice.  A row with entries whose
+    teacher logits are all -inf, or with an id outside the vocabulary, gives NaN.  ``n_valid`` (one float32 value on the device) replaces
+    the number of rows with entries."""
+    _check_logits(logits)
+    dev, V = logits.device, logits.shape[-1]
+    _need(top_ids.dim() == logits.dim() and top_ids.shape[-1] >= 1, f"top_ids: {tuple(logits.shape[:-1])} + [K] wanted, got {tuple(top_ids.shape)}")
+    K = top_ids.shape[-1]
+    _need(K <= MAX_TOP, f"top_ids: up to {MAX_TOP} entries a row, got {K}")
+    top_ids = _check_index(top_ids, (*logits.shape[:-1], K), "top_ids", dev)
+    _need(top_logits.shape == top_ids.shape and top_logits.device == dev, f"top_logits: {tuple(top_ids.shape)} on {dev} wanted, got {tuple(top_logits.shape)} on {top_logits.device}")
+    _need(top_logits.dtype in (torch.bfloat16, torch.float32), f"top_logits: bfloat16 or float32, got {top_logits.dtype}")
+    top_logits = top_logits.contiguous()
+    _need(temperature > 0 and math.isfinite(temperature), f"temperature: more than 0, got {temperature}")
+    n_valid = _check_n_valid(n_valid, dev)
+    grad = _gradient(logits, out, want_grad)
+    rows = logits.shape[:-1]
+    if not logits.is_cuda:
+        ids = top_ids.long()
+        keep, have = ids[..., 0] >= 0, (ids >= 0) & (ids < V)
+        bad = (ids >= V).any(-1) & keep
+        zero = torch.zeros((), dtype=torch.float64)
+        lq = torch.log_softmax(torch.where(have, top_logits.double() / temperature, torch.full((), -math.inf, dtype=torch.float64)), -1)
+        q = torch.where(have, lq.exp(), zero)
+        z, _, ls = _softmax64(logits.double() / temperature)
+        lp = z.gather(-1, ids.clamp(0, V - 1)) - ls[..., None]
+        kl = torch.where(have & (q != 0), q * (lq - lp), zero).sum(-1)
+        kl = torch.where(keep, torch.where(bad, torch.full_like(kl, math.nan), kl), zero)
+        w = 1.0 / (n_valid.double() if n_valid is not None else keep.sum().clamp(min=1).double())
+        if grad is not None:
+            d = torch.exp(z - ls[..., None])
+            d.scatter_add_(-1, ids.clamp(0, V - 1), -q)
+            d = torch.where(bad[..., None], torch.full_like(d, math.nan), d) * (temperature * w)
+            grad.copy_(torch.where(keep[..., None], d, zero).to(grad.dtype))
+        return DistillLoss((kl.sum() * temperature ** 2 * w).float().reshape(()), kl.float(), grad)
+    kl = _empty(dev, *rows)
+    T = kl.numel()
+    if not T:
+        return DistillLoss(torch.zeros((), device=dev), kl, grad)
+    loss, work = _empty(dev, 1), _empty(dev, T + 1)
+    arg = _Distill(top_ids.data_ptr(), top_logits.data_ptr(), int(top_ids.dtype == torch.int64), int(top_logits.dtype == torch.float32), K, float(temperature),
+                   ptr(n_valid), kl.data_ptr(), loss.data_ptr(), work.data_ptr() + 4 * T, work.data_ptr())
+    with _on(dev):
+        check(_lib.lib().tfb_distill_loss(_rows(logits, grad), arg, stream()), "distill_loss", 3)
+    return DistillLoss(loss[0], kl, grad)
+
+
+# ---------------------------------------------------------------------------------------------
+# scoring from hidden states
+# ---------------------------------------------------------------------------------------------
+SCORE_CHUNK = 1 << 28          # logits that exist at a time
+
+
+def linear_logprobs(x, weight, targets, ignore_index: int = -100):
+    """Log-probabilities of given tokens under a head, and the logsumexp of its logits, without all of the logits in memory: x [..., H], weight [V, H] (bfloat16, or
+    float32 on the CPU), targets of x's leading shape -> (logp, lse), float32, both 0 where the target is ``ignore_index``.  For passes that want
+    no gradient (reference models, older policies, evaluation); with one use ``token_logprobs`` on the logits."""
+    _need(not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)), "linear_logprobs has no gradient: call it under torch.no_grad(), or use token_logprobs")
+    _need(x.dim() >= 1 and weight.dim() == 2 and weight.shape[1] == x.shape[-1], f"x [..., H] and weight [V, H], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _need(x.dtype == weight.dtype, f"x and weight: one type, got {x.dtype} and {weight.dtype}")
+    _need(x.device == weight.device, f"weight: on {weight.device}, x is on {x.device}")
+    _need(weight.shape[0] > 0 and weight.shape[1] > 0, "an empty weight")
+    targets = _check_index(targets, x.shape[:-1], "targets", x.device)
+    x2, y = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
+    if not x.is_cuda:
+        _need(x.is_floating_point(), f"x: a floating type, got {x.dtype}")
+        keep, _, lp, (_, m, ls) = _taken(x2.float() @ weight.float().t(), y, ignore_index)
+        return lp.float().view(targets.shape), torch.where(keep, m + ls, torch.zeros((), dtype=m.dtype)).float().view(targets.shape)
+    _need(x.dtype == torch.bfloat16, f"x: bfloat16 on the GPU, got {x.dtype}")
+    _need(x.shape[-1] % 8 == 0, f"x: a width that is a multiple of 8, got {x.shape[-1]}")
+    ready = lambda t: t if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    x2, w = ready(x2), ready(weight)
+    lp, lse = _empty(x.device, y.numel()), _empty(x.device, y.numel())
+    with _on(x.device):
+        step = max(1, SCORE_CHUNK // w.shape[0])
+        for a in range(0, y.numel(), step):
+            part = slice(a, a + step)
+            _score_rows(F.gemm(x2[part], w, out_dtype=torch.float32), y[part], ignore_index, lp[part], lse[part], None)
+    return lp.view(targets.shape), lse.view(targets.shape)
