@@ -246,7 +246,9 @@ def test_policy(dev, dtype, lead, V, kw):
     near(o.logp, lp, lp_tol(lp) * (y != IGN), "logp")
     check_grad(o.dlogits, z, y, c, dtype)
     quiet = L.policy_loss_fwd_bwd(z, y, A, old, ref, want_grad=False, **kw)
-    assert quiet.dlogits is None and torch.equal(quiet.loss, o.loss) and torch.equal(quiet.logp, o.logp)
+    assert quiet.dlogits is None
+    near(quiet.loss, o.loss, 2 * slack, "loss without gradient")      # other groups of values are added up first: each of the two is within slack
+    near(quiet.logp, o.logp, 2 * lp_tol(lp) * (y != IGN))
     w = z.clone()
     again = L.policy_loss_fwd_bwd(w, y, A, old, ref, out=w, **kw)     # in place, and bit for bit again
     assert again.dlogits is w and torch.equal(w, o.dlogits) and torch.equal(again.loss, o.loss)

@@ -29,6 +29,7 @@ from . import _lib, functional as F
 from ._lib import c_f, c_i, c_ll, c_p, check, ptr, stream
 
 MAX_TOP = 1024          # entries of a teacher's row
+PIPE_CLUSTERS = 296     # most clusters of one launch, each with three sums of 8 bytes in the workspace
 
 _KL = {"k3": 0, "k1": 1}
 _MEAN = {"tokens": 0, "sequences": 1, "sum": 2}
@@ -36,23 +37,23 @@ _KIND = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 
 class _Rows(C.Structure):
-    _fields_ = [("z", c_p), ("dz", c_p), ("zb", c_ll), ("zs", c_ll), ("db", c_ll), ("ds", c_ll), ("T", c_i), ("S", c_i), ("V", c_i), ("f32", c_i)]
+    _fields_ = [("z", c_p), ("dz", c_p), ("zb", c_ll), ("zs", c_ll), ("db", c_ll), ("ds", c_ll), ("T", c_i), ("S", c_i), ("V", c_i), ("f32", c_i), ("status", c_p)]
 
 
 class _Policy(C.Structure):
     _fields_ = [("targets", c_p), ("idx64", c_i), ("ignore", c_ll), ("adv", c_p), ("old_lp", c_p), ("ref_lp", c_p), ("adv_seq", c_i), ("ratio", c_i),
                 ("kl_kind", c_i), ("mean", c_i), ("lo", c_f), ("hi", c_f), ("kl_coef", c_f), ("n_valid", c_p), ("logp", c_p), ("out", c_p),
-                ("denom", c_p), ("terms", c_p)]
+                ("ws", c_p), ("denom", c_p), ("counter", c_p)]
 
 
 class _Preference(C.Structure):
     _fields_ = [("targets", c_p), ("idx64", c_i), ("ignore", c_ll), ("ref", c_p), ("kind", c_i), ("average", c_i), ("beta", c_f), ("smooth", c_f),
-                ("loss", c_p), ("margins", c_p), ("logp", c_p), ("lp64", c_p), ("stats", c_p), ("coef", c_p), ("terms", c_p)]
+                ("loss", c_p), ("margins", c_p), ("logp", c_p), ("lp64", c_p), ("stats", c_p), ("coef", c_p), ("terms", c_p), ("counter", c_p)]
 
 
 class _Distill(C.Structure):
     _fields_ = [("top_ids", c_p), ("top_z", c_p), ("idx64", c_i), ("top_f32", c_i), ("K", c_i), ("tau", c_f), ("n_valid", c_p), ("kl", c_p), ("loss", c_p),
-                ("denom", c_p), ("terms", c_p)]
+                ("ws", c_p), ("denom", c_p), ("counter", c_p)]
 
 
 _lib.register("tfb_token_logprobs", [C.POINTER(_Rows), c_p, c_i, c_ll, c_p, c_p, c_p, c_p])
@@ -134,7 +135,8 @@ def _rows(logits, grad=None):
     strides = lambda t: (0, 0) if t is None else ((0, t.stride(0)) if two else (t.stride(0), t.stride(1)))
     zb, zs = strides(logits)
     db, ds = strides(grad)
-    return _Rows(logits.data_ptr(), ptr(grad), zb, zs, db, ds, T, max(S, 1), logits.shape[-1], int(logits.dtype == torch.float32))
+    return _Rows(logits.data_ptr(), ptr(grad), zb, zs, db, ds, T, max(S, 1), logits.shape[-1], int(logits.dtype == torch.float32),
+                 _lib.status_word(logits.device).data_ptr())
 
 
 def _on(device):
@@ -310,12 +312,15 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     if not lp.numel():
         z = torch.zeros((), device=dev)
         return PolicyLoss(z, z, z, lp, grad)
-    sums, work = _empty(dev, 3), _empty(dev, 3 * lp.numel() + max(1, B))
+    T = lp.numel()
+    n_ws = max(3 * T, 6 * min(T, PIPE_CLUSTERS))
+    sums, work = _empty(dev, 3), _empty(dev, n_ws + B + 1)
+    ws = work.data_ptr()
     arg = _Policy(targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), advantages.data_ptr(), ptr(old), ptr(ref), int(adv_seq), int(ratio),
                   _KL[kl], _MEAN[mean], 1 - lo, 1 + hi, float(kl_coef), ptr(n_valid), lp.data_ptr(), sums.data_ptr(),
-                  work.data_ptr() + 12 * lp.numel(), work.data_ptr())
+                  ws, ws + 4 * n_ws, ws + 4 * (n_ws + B))
     with _on(dev):
-        check(_lib.lib().tfb_policy_loss(_rows(logits, grad), arg, stream()), "policy_loss", 3)
+        check(_lib.lib().tfb_policy_loss(_rows(logits, grad), arg, stream()), "policy_loss", 2)
     return PolicyLoss(sums[0], sums[1], sums[2], lp, grad)
 
 
@@ -375,12 +380,12 @@ def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float =
         l = {"sigmoid": torch.nn.functional.softplus(-x) + label_smoothing * x, "hinge": (1 - x).clamp(min=0), "squared": (x / beta - 0.5 / beta) ** 2}[kind]
         return PreferenceLoss(l.sum() / max(N, 1), x, L, grad)
     T = 2 * N * S
-    loss, lp64, work = _empty(dev, 1), _empty(dev, T, dtype=torch.float64), _empty(dev, 2 * T + 3 * N)
+    loss, lp64, work = _empty(dev, 1), _empty(dev, T, dtype=torch.float64), _empty(dev, 2 * T + 3 * N + 1)
     arg = _Preference(targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), ptr(ref), _KIND[kind], int(average), float(beta),
                       float(label_smoothing), loss.data_ptr(), margins.data_ptr(), L.data_ptr(), lp64.data_ptr(), work.data_ptr(),
-                      work.data_ptr() + 8 * T, work.data_ptr() + 8 * T + 8 * N)
+                      work.data_ptr() + 8 * T, work.data_ptr() + 8 * T + 8 * N, work.data_ptr() + 8 * T + 12 * N)
     with _on(dev):
-        check(_lib.lib().tfb_preference_loss(_rows(logits, grad), arg, stream()), "preference_loss", 4 if want_grad else 3)
+        check(_lib.lib().tfb_preference_loss(_rows(logits, grad), arg, stream()), "preference_loss", 3 if want_grad else 2)
     return PreferenceLoss(loss[0], margins, L, grad)
 
 
@@ -437,11 +442,13 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     T = kl.numel()
     if not T:
         return DistillLoss(torch.zeros((), device=dev), kl, grad)
-    loss, work = _empty(dev, 1), _empty(dev, T + 1)
+    n_ws = max(T, 6 * min(T, PIPE_CLUSTERS))
+    loss, work = _empty(dev, 1), _empty(dev, n_ws + 2)
+    ws = work.data_ptr()
     arg = _Distill(top_ids.data_ptr(), top_logits.data_ptr(), int(top_ids.dtype == torch.int64), int(top_logits.dtype == torch.float32), K, float(temperature),
-                   ptr(n_valid), kl.data_ptr(), loss.data_ptr(), work.data_ptr() + 4 * T, work.data_ptr())
+                   ptr(n_valid), kl.data_ptr(), loss.data_ptr(), ws, ws + 4 * n_ws, ws + 4 * n_ws + 4)
     with _on(dev):
-        check(_lib.lib().tfb_distill_loss(_rows(logits, grad), arg, stream()), "distill_loss", 3)
+        check(_lib.lib().tfb_distill_loss(_rows(logits, grad), arg, stream()), "distill_loss", 2)
     return DistillLoss(loss[0], kl, grad)
 
 
