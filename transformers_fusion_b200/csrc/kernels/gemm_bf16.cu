@@ -91,6 +91,10 @@ struct GemmParams {
   int glu;       // pair form: > 0: the first CTA's 128 columns of B are rows n of W, the second's rows glu + n; C = act(first) * second
   int c_tma;     // 1: the epilogue goes through shared memory and the C tensor map (aligned, dense C)
   int* status;
+  // row statistics instead of C: part[i * part_ld + row] = (m, sum exp(c - m)) over the i-th half tile of that row's columns
+  float2* part;
+  long long part_ld;
+  const int* rows;     // device: rows of A that hold anything, at most M
 };
 
 // Decodes work item w into tile coordinates / k-block range / expert.  Returns false when there is nothing to do.
@@ -416,7 +420,51 @@ __device__ __forceinline__ void glu_epilogue(const GemmParams& p, const CUtensor
   }
 }
 
-template <bool A_MN, bool B_MN, int BN>
+// Maximum and sum of exponentials of a row's columns in half a tile, one row to a thread: the product itself stays in tensor memory.
+template <int BN>
+__device__ __forceinline__ void stats_epilogue(const GemmParams& p, uint32_t taddr0, int n0, int row, int half) {
+  constexpr float LOG2E = 1.4426950408889634f;
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < BN / 64; ++c) {
+    const int col0 = n0 + half * (BN / 2) + c * 32;
+    if (col0 >= p.N) break;
+    uint32_t r[32];
+    tmem_ld_32x32(taddr0 + half * (BN / 2) + c * 32, r);
+    tmem_ld_wait();
+    if (col0 + 32 > p.N) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j >= p.N) r[j] = 0xff800000u;      // -inf
+    }
+    float a[11];
+#pragma unroll
+    for (int j = 0; j < 10; ++j) a[j] = fmax3(__uint_as_float(r[3 * j]), __uint_as_float(r[3 * j + 1]), __uint_as_float(r[3 * j + 2]));
+    a[10] = fmax3(__uint_as_float(r[30]), __uint_as_float(r[31]), m);
+    const float mx = fmax3(fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmax3(a[6], a[7], a[8])), a[9], a[10]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float2 neg = make_float2(-ref, -ref), k2 = make_float2(LOG2E, LOG2E);
+    float2 t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float2 d = mul2(add2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), neg), k2);
+      float2 e;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(d.x));
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(d.y));
+      t[(j >> 1) & 3] = add2(t[(j >> 1) & 3], e);
+    }
+    const float2 u = add2(add2(t[0], t[1]), add2(t[2], t[3]));
+    float old;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(old) : "f"((m - ref) * LOG2E));
+    s = fmaf(s, old, u.x + u.y);
+    m = mx;
+  }
+  if (row < p.M) p.part[(n0 / (BN / 2) + half) * p.part_ld + row] = make_float2(m, s);
+}
+
+template <bool A_MN, bool B_MN, int BN, bool STATS = false>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_c, const __grid_constant__ PeerMaps tma_peers, const GemmParams p) {
@@ -619,6 +667,14 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       tc_fence_after();
       const int row = m0 + quad * 32 + lane;
       const uint32_t taddr0 = tmem_base + abuf * BN + (uint32_t(quad * 32) << 16);
+      if constexpr (STATS) {
+        stats_epilogue<BN>(p, taddr0, n0, row, half);
+        tc_fence_before();
+        mbar_arrive(bar_tempty + abuf * 8);
+        abuf ^= 1;
+        if (abuf == 0) aphase ^= 1;
+        continue;
+      }
       if (p.c_tma) {
         staged_epilogue<BN, L::STG_BUFS>(p, tma_c, tma_peers, taddr0, n0, m0 + quad * 32, half, lane, stg_u32, sbuf,
                                          p.group_mode == 2 ? it.expert : 0);
@@ -754,7 +810,7 @@ struct PairSmem {
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
 };
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool STATS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const __grid_constant__ CUtensorMap tma_c,
                  const __grid_constant__ PeerMaps tma_peers, const GemmParams p) {
@@ -801,11 +857,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   tfb::pdl_sync();
 
   const int total_kb = (p.K + BK - 1) / BK;
-  const int num_work = p.tiles_m * p.tiles_n * p.splits;
+  const int tiles_m = STATS ? (*p.rows + 2 * BM - 1) / (2 * BM) : p.tiles_m;
+  const int num_work = tiles_m * p.tiles_n * p.splits;
   // work item -> tile (grouped raster, see decode_work) and k-blocks
   auto decode = [&](int w, int& m0, int& n0, int& kb0, int& kb1) {
     const int tile = w / p.splits, split = w - tile * p.splits;
-    const int per_group = p.raster_gn * p.tiles_m;
+    const int per_group = p.raster_gn * tiles_m;
     const int grp = tile / per_group, within = tile - grp * per_group;
     const int gn = min(p.raster_gn, p.tiles_n - grp * p.raster_gn);
     const int mi = within / gn;
@@ -895,7 +952,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       if (!mbar_wait_warp(bar_tfull + abuf * 8, aphase, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL)) break;
       tc_fence_after();
       const uint32_t taddr0 = tmem_base + abuf * BN + (uint32_t(quad * 32) << 16);
-      if (p.glu) glu_epilogue(p, tma_c, taddr0, n0, m0 + quad * 32, half, lane, stg_u32);
+      if constexpr (STATS) stats_epilogue<BN>(p, taddr0, n0, m0 + quad * 32 + lane, half);
+      else if (p.glu) glu_epilogue(p, tma_c, taddr0, n0, m0 + quad * 32, half, lane, stg_u32);
       else staged_epilogue<BN, L::STG_BUFS>(p, tma_c, tma_peers, taddr0, n0, m0 + quad * 32, half, lane, stg_u32, sbuf, 0);
       tc_fence_before();
       __syncwarp();
@@ -917,23 +975,23 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
 // -------------------------------------------------------------------------------------------------
 // host launcher
 // -------------------------------------------------------------------------------------------------
-template <bool A_MN, bool B_MN, int BN>
+template <bool A_MN, bool B_MN, int BN, bool STATS = false>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const PeerMaps& tpeers, const GemmParams& p,
                   int grid, cudaStream_t st) {
   using L = SmemLayout<BN>;
   static DeviceOnce once;
-  auto kern = gemm_bf16_kernel<A_MN, B_MN, BN>;
+  auto kern = gemm_bf16_kernel<A_MN, B_MN, BN, STATS>;
   if (int e = ensure_dyn_smem(once, kern, L::TOTAL)) return e;
   tfb::launch_k(kern, grid, GEMM_THREADS, L::TOTAL, st, ta, tb, tc, tpeers, p);
   return int(cudaGetLastError());
 }
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool STATS = false>
 static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const GemmParams& p, int pairs, cudaStream_t st) {
   using L = PairSmem;
   static DeviceOnce once;
   static const PeerMaps none = {};
-  auto kern = gemm_pair_kernel<A_MN, B_MN>;
+  auto kern = gemm_pair_kernel<A_MN, B_MN, STATS>;
   if (int e = ensure_dyn_smem(once, kern, L::TOTAL)) return e;
   tfb::launch_k(kern, 2 * pairs, GEMM_THREADS, L::TOTAL, st, ta, tb, tc, none, p);
   return int(cudaGetLastError());
@@ -1360,6 +1418,42 @@ TFB_API int tfb_gemm_glu(const void* A, long long lda, const void* B, long long 
   p.splits = 1;
   p.kb_per_split = (K + BK - 1) / BK;
   return launch_pair<false, false>(ta, tb, tc, p, min(p.tiles_m * p.tiles_n, sm_count() / 2), static_cast<cudaStream_t>(stream));
+}
+
+// Statistics of the rows of A . B^T without the product in memory (see GemmParams::part): A [M, K] of which the first *rows rows count, B [N, K].  Returns the
+// number of parts of a row (`part` holds that many x M entries, at most 2 ceil(N / 128)), or an error.
+// Up to one tile of rows B is streamed once, in tiles of 128 columns on single CTAs: SMEMNOTE
+int tfb::gemm_row_stats(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const int* rows, float2* part, int* status,
+                        void* stream) {
+  CUtensorMap ta, tb;
+  if (M <= 0 || N <= 0 || K <= 0) return TFB_ERR_ARG;
+  GemmParams p = {};
+  p.M = M; p.N = N; p.K = K;
+  p.alpha = 1.f;
+  p.num_experts = 1; p.rs_world = 1;
+  p.status = status;
+  p.part = part; p.part_ld = M; p.rows = rows;
+  p.splits = 1;
+  p.kb_per_split = (K + BK - 1) / BK;
+  p.wg_n_shift = -1;
+  const bool one = M <= BM || sm_count() < 2;
+  if (int rc = make_tmap_2d(&ta, A, 2, K, M, lda * 2, BK, BM)) return rc;
+  const int rows_of_tile = one ? BM : 2 * BM, cols_of_tile = one ? BM : 2 * BM;
+  p.tiles_m = (M + rows_of_tile - 1) / rows_of_tile;
+  p.tiles_n = (N + cols_of_tile - 1) / cols_of_tile;
+  p.raster_gn = p.tiles_n > 12 && p.tiles_m >= 2 ? 8 : p.tiles_n;
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc;
+  if (one) {
+    static const PeerMaps none = {};
+    if ((rc = make_tmap_3d(&tb, B, 2, K, N, 1, ldb * 2, (unsigned long long)ldb * 2 * N, BK, BM, 1))) return rc;
+    rc = launch<false, false, BM, true>(ta, tb, ta, none, p, int(min(tiles, (long long)sm_count())), st);
+  } else {
+    if ((rc = make_tmap_2d(&tb, B, 2, K, N, ldb * 2, BK, BM))) return rc;
+    rc = launch_pair<false, false, true>(ta, tb, ta, p, int(min(tiles, (long long)sm_count() / 2)), st);
+  }
+  return rc ? (rc > 0 ? -1000 - rc : rc) : 2 * p.tiles_n;
 }
 
 // The same for weights of a model that serves: the caller promises that the kernel launched just before this one on the stream does not

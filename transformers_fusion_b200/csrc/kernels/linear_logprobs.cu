@@ -1,0 +1,198 @@
+// Log-probabilities of given tokens under a head, from hidden states: lp = x . w[y] - log sum_v exp(x . w[v]), without the [T, V] logits in memory.
+//
+//   gather   rows that are scored, one behind the other: a prompt's rows take no part in the product
+//   product  x W^T on tensor cores (gemm_bf16.cu), whose epilogue keeps (m, sum exp) of every row's columns in half a tile and drops the rest
+//   finish   joins a row's parts (or takes its statistics), and takes the product with its target's row of W by itself, in 32-bit fused multiply-adds: the tensor cores'
+//            accumulation is off by a few 2^-24 of the partial sums at each of its steps, in one direction, which the log of a sum over
+//            thousands of columns does not show but the one value that is subtracted from it does (relative error of lp at 4096 terms 1.3e-6 against 2.6e-7)
+#include "tfb_host.h"
+#include "tfb_ptx.cuh"
+
+TFB_BOUNDS_DEFINE(linear_logprobs)
+
+namespace tfb {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ long long ld_idx(const void* p, long long i, int is64) {
+  return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+}
+
+struct ScoreArg {
+  const __nv_bfloat16 *x, *w;
+  long long ldx, ldw;
+  const void* targets;
+  int idx64;
+  long long ignore;
+  int M, V, H;
+  float *logp, *lse;                   // [M]
+  int* rows;                           // one word, 0 before the launch: rows that are scored
+  int* row_of;                         // [M]
+  __nv_bfloat16* xc;                   // [M, ldc]: their hidden states
+  long long ldc;
+  float2* part;                        // [2 ceil(V / 128), M]
+  int parts;                           // of a row; set by the launch
+  float* z;                            // few rows, else null: [M, ldz] logits, ldz a multiple of 4
+  long long ldz;
+  float* stats;                        // few rows: [2, M]
+};
+
+constexpr int GATHER_ROWS = 32;
+
+// Which place a row gets depends on the order in which blocks arrive; what is computed for it does not.
+__global__ void __launch_bounds__(256) score_gather_kernel(const ScoreArg a) {
+  tfb::pdl_sync();
+  __shared__ int place[GATHER_ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * GATHER_ROWS;
+  if (warp == 0) {
+    const int row = r0 + lane;
+    const bool on = row < a.M && ld_idx(a.targets, row, a.idx64) != a.ignore;
+    const unsigned mask = __ballot_sync(~0u, on);
+    int base = 0;
+    if (lane == 0 && mask) base = atomicAdd(a.rows, __popc(mask));
+    base = __shfl_sync(~0u, base, 0);
+    const int at = base + __popc(mask & ((1u << lane) - 1));
+    place[lane] = on ? at : -1;
+    if (on) a.row_of[at] = row;
+    else if (row < a.M) a.logp[row] = a.lse[row] = 0.f;
+  }
+  __syncthreads();
+  for (int i = warp; i < GATHER_ROWS; i += 8) {
+    const int at = place[i];
+    if (at < 0) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(a.x + (r0 + i) * a.ldx);
+    uint4* dst = reinterpret_cast<uint4*>(a.xc + at * a.ldc);
+    for (int v = lane; v < a.H / 8; v += 32) dst[v] = src[v];
+  }
+}
+
+// x[row] . w[target] by a warp; NaN for a target outside the vocabulary
+__device__ __forceinline__ float target_logit(const ScoreArg& a, long long row, int lane) {
+  const long long y = ld_idx(a.targets, row, a.idx64);
+  const bool in = y >= 0 && y < a.V;
+  if (lane == 0) TFB_BOUNDS(in, 3, y, a.V);
+  float z = NAN;                     // a target outside the vocabulary
+  if (in) {
+    const uint4 *p = reinterpret_cast<const uint4*>(a.x + row * a.ldx), *q = reinterpret_cast<const uint4*>(a.w + y * a.ldw);
+    float2 t = make_float2(0.f, 0.f), u = t;
+#pragma unroll 4
+    for (int v = lane; v < a.H / 8; v += 32) {
+      const uint4 f = p[v], g = q[v];
+      t = fma2(unpack_bf16(f.x), unpack_bf16(g.x), t);
+      u = fma2(unpack_bf16(f.y), unpack_bf16(g.y), u);
+      t = fma2(unpack_bf16(f.z), unpack_bf16(g.z), t);
+      u = fma2(unpack_bf16(f.w), unpack_bf16(g.w), u);
+    }
+    z = (t.x + u.x) + (t.y + u.y);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(~0u, z, o);
+  }
+  return z;
+}
+
+// R rows to a block, 256 / R threads to a row's parts, eight loads under way in each.  Four rows (of which a part's entries are one 32-byte sector) while
+// there are few: a row of a vocabulary of 128256 has 2004 parts, which take sixteen threads 75 us one by one.
+template <int R>
+__global__ void __launch_bounds__(256) score_finish_kernel(const ScoreArg a) {
+  tfb::pdl_sync();
+  constexpr int SHARES = 256 / R, U = 8;
+  const int n = *a.rows, r0 = blockIdx.x * R;
+  if (r0 >= n) return;
+  __shared__ float2 sh[SHARES][R];
+  __shared__ float zy[R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  {
+    const int i = threadIdx.x % R, share = threadIdx.x / R, at = min(r0 + i, n - 1);
+    float m = -INFINITY, s = 0.f;
+    for (int p = share; p < a.parts; p += SHARES * U) {
+      float2 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = p + u * SHARES < a.parts ? a.part[(long long)(p + u * SHARES) * a.M + at] : make_float2(-INFINITY, 0.f);
+      float M = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) M = fmaxf(M, v[u].x);
+      const float r = M == -INFINITY ? 0.f : M;
+      s *= ex2((m - r) * LOG2E);
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += v[u].y * ex2((v[u].x - r) * LOG2E);
+      m = M;
+    }
+    sh[share][i] = make_float2(m, s);
+  }
+  for (int i = warp; i < R && r0 + i < n; i += 8) {
+    const int row = a.row_of[r0 + i];
+    const float z = target_logit(a, row, lane);
+    if (lane == 0) zy[i] = z;
+  }
+  __syncthreads();
+  // one warp to a row: its shares in 64 bits
+  for (int i = warp; i < R && r0 + i < n; i += 8) {
+    float m = -INFINITY;
+    for (int j = lane; j < SHARES; j += 32) m = fmaxf(m, sh[j][i].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float r = m == -INFINITY ? 0.f : m;
+    double s = 0.0;
+    for (int j = lane; j < SHARES; j += 32) s += double(sh[j][i].y * ex2((sh[j][i].x - r) * LOG2E));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    if (lane) continue;
+    const double ls = log(s), lp = double(zy[i]) - double(m) - ls;
+    const int row = a.row_of[r0 + i];
+    a.lse[row] = float(double(m) + ls);
+    a.logp[row] = lp > 0.0 ? 0.f : float(lp);      // the two products' roundings are not the same
+  }
+}
+
+// The same for rows whose statistics are there: a warp to a row.
+__global__ void __launch_bounds__(256) score_rows_kernel(const ScoreArg a) {
+  tfb::pdl_sync();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.M) return;
+  const bool on = ld_idx(a.targets, row, a.idx64) != a.ignore;
+  const float z = on ? target_logit(a, row, lane) : 0.f;
+  if (lane) return;
+  const double m = a.stats[row], ls = a.stats[a.M + row], lp = double(z) - m - ls;
+  a.lse[row] = float(m + ls);
+  a.logp[row] = lp > 0.0 ? 0.f : float(lp);
+}
+
+}  // namespace tfb
+
+using namespace tfb;
+
+// x [M, H] and w [V, H] bf16, pitches multiples of 8, 16-byte aligned; H a multiple of 8.  Writes all of the workspace that it reads.
+TFB_API int tfb_linear_logprobs(const ScoreArg* p, int* status, void* stream) {
+  if (!p || !p->x || !p->w || !p->targets || !p->logp || !p->lse || !p->rows || !p->row_of || !p->xc || !p->part || p->M <= 0 || p->V <= 0 || p->H <= 0 || p->H % 8 ||
+      p->ldx % 8 || p->ldw % 8 || p->ldc % 8 || ((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->w) | reinterpret_cast<uintptr_t>(p->xc)) & 15))
+    return TFB_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Few rows: the weights are streamed once, which the products of a decode step do nearer to the memory's rate than the epilogue's kernel (its tiles are
+  // too few rows high to keep enough of W under way), and the logits stay in L2.  us, this way / that kernel, rows x V x H: 1 x 128256 x 4096 165 / 298, 61 x 128256 x 4096
+  // 183 / 216, 128 x 128256 x 4096 213 / 222, 61 x 32000 x 512 21.2 / 23.4, but 128 x 32000 x 512 28 / 21 and 128 x 128256 x 512 71 / 45.
+  if (p->z && (p->M <= 64 || (p->M <= 128 && p->H >= 2048))) {
+    if (!p->stats || p->ldz % 4 || (reinterpret_cast<uintptr_t>(p->z) & 15)) return TFB_ERR_ARG;
+    int rc = gemm_skinny(p->x, p->ldx, p->w, p->ldw, p->z, p->ldz, p->M, p->V, p->H, nullptr, nullptr, 0, 1.f, 0, 1, stream);
+    if (rc == TFB_NOT_TAKEN)
+      rc = gemm_rows(p->x, p->ldx, p->w, p->ldw, nullptr, nullptr, -1, 0, p->z, p->ldz, p->M, p->V, p->H, p->H, nullptr, nullptr, 0, 1.f, 0, 1, 0, status, stream);
+    if (rc != TFB_NOT_TAKEN) {
+      if (!rc) rc = row_stats(p->z, p->ldz, p->M, p->V, p->targets, p->idx64, p->ignore, p->stats, status, stream);
+      if (rc) return rc;
+      tfb::launch_k_rows(p->M, score_rows_kernel, (p->M + 7) / 8, 256, 0, st, *p);
+      return int(cudaGetLastError());
+    }
+  }
+  if (cudaError_t e = cudaMemsetAsync(p->rows, 0, sizeof(int), st)) return int(e);
+  tfb::launch_k(score_gather_kernel, (p->M + GATHER_ROWS - 1) / GATHER_ROWS, 256, 0, st, *p);
+  ScoreArg a = *p;
+  a.parts = gemm_row_stats(p->xc, p->ldc, p->w, p->ldw, p->M, p->V, p->H, p->rows, p->part, status, stream);
+  if (a.parts <= 0) return a.parts <= -1000 ? -1000 - a.parts : a.parts;
+  if (p->M <= 2048) tfb::launch_k(score_finish_kernel<4>, (p->M + 3) / 4, 256, 0, st, a);
+  else tfb::launch_k(score_finish_kernel<16>, (p->M + 15) / 16, 256, 0, st, a);
+  return int(cudaGetLastError());
+}

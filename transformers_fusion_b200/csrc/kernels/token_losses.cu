@@ -44,7 +44,6 @@ struct LossArg {
   // statistics
   float* logp;                         // [T]
   float* stats;                        // [2, T]: m and log S apart, since their sum in 32 bits loses log S where |m| is large; MODE_GRAD reads them
-  float* lse;                          // [T] or null: the sum
   double* logp64;                      // [T], preference
   // MODE_GRAD: coefficient of a row
   const float* dlogp;                  // [T], or [T / S] with per_seq
@@ -146,7 +145,6 @@ __device__ __forceinline__ void put_stats(const LossArg& a, int T, long long t, 
   if (MODE != MODE_GRAD && a.logp) a.logp[t] = float(lp);
   if (MODE != MODE_STATS) return;
   if (a.logp64) a.logp64[t] = lp;
-  if (a.lse) a.lse[t] = float(double(m) + ls);
   if (a.stats) {
     a.stats[t] = m;
     a.stats[T + t] = float(ls);
@@ -1165,18 +1163,26 @@ static int rows_and_sums(const RowsArg& r, LossArg a, int nsums, void* ws, int* 
   return int(cudaGetLastError());
 }
 
+int row_stats(const float* z, long long ldz, int T, int V, const void* targets, int idx64, long long ignore, float* stats, int* status, void* stream) {
+  RowsArg r = {};
+  r.z = z; r.zs = ldz; r.T = r.S = T; r.V = V; r.f32 = 1; r.status = status;
+  LossArg a = {};
+  a.targets = targets; a.idx64 = idx64; a.ignore = ignore; a.stats = stats;
+  return rows_and_sums<MODE_STATS>(r, a, 0, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
 static bool bad_rows(const RowsArg& r) { return !r.z || r.T <= 0 || r.S <= 0 || r.V <= 0 || r.T % r.S; }
 
 }  // namespace tfb
 
 using namespace tfb;
 
-// logp, lse [T], stats [2, T] (each may be null); 0 where the target is `ignore`.
-TFB_API int tfb_token_logprobs(const RowsArg* r, const void* targets, int idx64, long long ignore, float* logp, float* lse, float* stats, void* stream) {
-  if (!r || bad_rows(*r) || !targets) return TFB_ERR_ARG;
+// logp [T], stats [2, T]; 0 where the target is `ignore`.
+TFB_API int tfb_token_logprobs(const RowsArg* r, const void* targets, int idx64, long long ignore, float* logp, float* stats, void* stream) {
+  if (!r || bad_rows(*r) || !targets || !logp || !stats) return TFB_ERR_ARG;
   LossArg a = {};
   a.targets = targets; a.idx64 = idx64; a.ignore = ignore;
-  a.logp = logp; a.lse = lse; a.stats = stats;
+  a.logp = logp; a.stats = stats;
   RowsArg rows = *r;
   rows.dz = nullptr;
   return rows_and_sums<MODE_STATS>(rows, a, 0, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));

@@ -77,7 +77,7 @@ def bounds_report(reset: bool = True) -> dict:
         return out
     for unit in ("elementwise", "loss_optim", "moe_routing", "gemm_bf16", "fsdp_fused", "loss_vocab_parallel", "ep_fused",
                  "paged_attention", "stack_ops", "streams", "delta_rule", "diff_attention", "head_attention", "latent_attention", "gated_linear", "moe_serve",
-                 "token_losses"):
+                 "token_losses", "linear_logprobs"):
         fn = getattr(lib(), f"tfb_bounds_report_{unit}", None)
         if fn is None:
             continue

@@ -18,109 +18,107 @@ logits themselves, which are then overwritten; None makes a new one.  Per-row re
 Reference counterparts: log-probabilities, ratio clipping and KL terms of the RL trainers (src/trainer/trainer_rl.cpp:557-1350)."""
 from __future__ import annotations
 
-import contextlib
-import ctypes as C
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
-from . import _lib, functional as F
-from ._lib import c_f, c_i, c_ll, c_p, check, ptr, stream
+from . import _lib
+from ._lib import c_i, c_ll, c_p, check
 
 MAX_TOP = 1024          # entries of a teacher's row
 PIPE_CLUSTERS = 296     # most clusters of one launch, each with three sums of 8 bytes in the workspace
+SCORE_ROWS = 1 << 15    # rows of one launch of linear_logprobs: bounds its workspace (a row's hidden state, and 8 bytes per 128 of the vocabulary)
 
 _KL = {"k3": 0, "k1": 1}
 _MEAN = {"tokens": 0, "sequences": 1, "sum": 2}
 _KIND = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
+# Arguments of the C entry points travel as packed structures (natural alignment, as the compiler lays them out): a call of a small loss is a few
+# microseconds of GPU time, and a ctypes structure of twenty fields would cost as much again.
+_ROWS = struct.Struct("@PPqqqqiiiiP0P")                      # z, dz, zb, zs, db, ds, T, S, V, f32, status
+_POLICY = struct.Struct("@PiqPPPiiiifffPPPPPP0P")            # targets, idx64, ignore, adv, old, ref, adv_seq, ratio, kl, mean, lo, hi, kl_coef, n_valid, logp, out, ws, denom, counter
+_PREFERENCE = struct.Struct("@PiqPiiffPPPPPPPP0P")           # targets, idx64, ignore, ref, kind, average, beta, smooth, loss, margins, logp, lp64, stats, coef, terms, counter
+_DISTILL = struct.Struct("@PPiiifPPPPPP0P")                  # ids, z, idx64, top_f32, K, tau, n_valid, kl, loss, ws, denom, counter
+_SCORE = struct.Struct("@PPqqPiqiiiPPPPPqPiPqP0P")           # x, w, ldx, ldw, targets, idx64, ignore, M, V, H, logp, lse, rows, row_of, xc, ldc, part, parts, z, ldz, stats
 
-class _Rows(C.Structure):
-    _fields_ = [("z", c_p), ("dz", c_p), ("zb", c_ll), ("zs", c_ll), ("db", c_ll), ("ds", c_ll), ("T", c_i), ("S", c_i), ("V", c_i), ("f32", c_i), ("status", c_p)]
-
-
-class _Policy(C.Structure):
-    _fields_ = [("targets", c_p), ("idx64", c_i), ("ignore", c_ll), ("adv", c_p), ("old_lp", c_p), ("ref_lp", c_p), ("adv_seq", c_i), ("ratio", c_i),
-                ("kl_kind", c_i), ("mean", c_i), ("lo", c_f), ("hi", c_f), ("kl_coef", c_f), ("n_valid", c_p), ("logp", c_p), ("out", c_p),
-                ("ws", c_p), ("denom", c_p), ("counter", c_p)]
-
-
-class _Preference(C.Structure):
-    _fields_ = [("targets", c_p), ("idx64", c_i), ("ignore", c_ll), ("ref", c_p), ("kind", c_i), ("average", c_i), ("beta", c_f), ("smooth", c_f),
-                ("loss", c_p), ("margins", c_p), ("logp", c_p), ("lp64", c_p), ("stats", c_p), ("coef", c_p), ("terms", c_p), ("counter", c_p)]
-
-
-class _Distill(C.Structure):
-    _fields_ = [("top_ids", c_p), ("top_z", c_p), ("idx64", c_i), ("top_f32", c_i), ("K", c_i), ("tau", c_f), ("n_valid", c_p), ("kl", c_p), ("loss", c_p),
-                ("ws", c_p), ("denom", c_p), ("counter", c_p)]
-
-
-_lib.register("tfb_token_logprobs", [C.POINTER(_Rows), c_p, c_i, c_ll, c_p, c_p, c_p, c_p])
-_lib.register("tfb_token_logprobs_bwd", [C.POINTER(_Rows), c_p, c_i, c_ll, c_p, c_p, c_p])
-_lib.register("tfb_policy_loss", [C.POINTER(_Rows), C.POINTER(_Policy), c_p])
-_lib.register("tfb_preference_loss", [C.POINTER(_Rows), C.POINTER(_Preference), c_p])
-_lib.register("tfb_distill_loss", [C.POINTER(_Rows), C.POINTER(_Distill), c_p])
+_lib.register("tfb_token_logprobs", [c_p, c_p, c_i, c_ll, c_p, c_p, c_p])
+_lib.register("tfb_token_logprobs_bwd", [c_p, c_p, c_i, c_ll, c_p, c_p, c_p])
+_lib.register("tfb_policy_loss", [c_p, c_p, c_p])
+_lib.register("tfb_preference_loss", [c_p, c_p, c_p])
+_lib.register("tfb_distill_loss", [c_p, c_p, c_p])
+_lib.register("tfb_linear_logprobs", [c_p, c_p, c_p])
 
 
 # ---------------------------------------------------------------------------------------------
 # arguments
 # ---------------------------------------------------------------------------------------------
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
-
-
-def _check_logits(logits, name="logits"):
-    _need(logits.dim() in (2, 3), f"{name}: [T, V] or [B, S, V], got {tuple(logits.shape)}")
-    _need(logits.dtype in (torch.bfloat16, torch.float32), f"{name}: bfloat16 or float32, got {logits.dtype}")
-    _need(logits.shape[-1] > 0, f"{name}: an empty vocabulary")
-    _need(logits.stride(-1) == 1 or logits.shape[-1] == 1, f"{name}: the last dimension has to be dense")
+def _check_logits(logits):
+    if logits.dim() not in (2, 3):
+        raise ValueError(f"logits: [T, V] or [B, S, V], got {tuple(logits.shape)}")
+    if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
+        raise ValueError(f"logits: bfloat16 or float32, got {logits.dtype}")
+    if logits.shape[-1] == 0:
+        raise ValueError("logits: an empty vocabulary")
+    if logits.stride(-1) != 1 and logits.shape[-1] != 1:
+        raise ValueError("logits: the last dimension has to be dense")
 
 
 def _check_index(idx, shape, name, device):
-    _need(idx.dtype in (torch.int64, torch.int32), f"{name}: int64 or int32, got {idx.dtype}")
-    _need(tuple(idx.shape) == tuple(shape), f"{name}: {tuple(shape)} wanted, got {tuple(idx.shape)}")
-    _need(idx.device == device, f"{name}: on {idx.device}, the logits are on {device}")
-    return idx.contiguous()
+    if idx.dtype is not torch.int64 and idx.dtype is not torch.int32:
+        raise ValueError(f"{name}: int64 or int32, got {idx.dtype}")
+    if idx.shape != shape or idx.device != device:
+        raise ValueError(f"{name}: {tuple(shape)} on {device} wanted, got {tuple(idx.shape)} on {idx.device}")
+    return idx if idx.is_contiguous() else idx.contiguous()
 
 
 def _check_f32(t, shape, name, device):
     """A float32 tensor of this shape, dense; None stays None."""
     if t is None:
         return None
-    _need(t.dtype == torch.float32, f"{name}: float32, got {t.dtype}")
-    _need(tuple(t.shape) == tuple(shape), f"{name}: {tuple(shape)} wanted, got {tuple(t.shape)}")
-    _need(t.device == device, f"{name}: on {t.device}, the logits are on {device}")
-    return t.contiguous()
+    if t.dtype is not torch.float32 or t.shape != shape or t.device != device:
+        raise ValueError(f"{name}: float32 {tuple(shape)} on {device} wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_n_valid(n_valid, device):
     if n_valid is None:
         return None
-    _need(n_valid.numel() == 1, "n_valid: one value")
-    return _check_f32(n_valid.reshape(1), (1,), "n_valid", device)
+    if n_valid.numel() != 1:
+        raise ValueError("n_valid: one value")
+    return _check_f32(n_valid.reshape(1), torch.Size((1,)), "n_valid", device)
+
+
+def _one_of(value, choices, name):
+    if value not in choices:
+        raise ValueError(f"{name}: one of {sorted(choices)}, got {value!r}")
+    return choices[value]
 
 
 def _gradient(logits, out, want_grad):
     """Where the gradient goes: None, ``out``, or a new tensor."""
     if not want_grad:
-        _need(out is None, "out: without want_grad there is no gradient")
+        if out is not None:
+            raise ValueError("out: without want_grad there is no gradient")
         return None
     if out is None:
-        # rows of the same alignment as those of the logits where they are dense
-        return torch.empty_like(logits, memory_format=torch.preserve_format)
-    _need(out.shape == logits.shape and out.dtype == logits.dtype and out.device == logits.device, "out: the logits' shape, type and device")
-    _need(out.stride(-1) == 1 or out.shape[-1] == 1, "out: the last dimension has to be dense")
-    V, dims = out.shape[-1], sorted((out.stride(i), out.shape[i]) for i in range(out.dim() - 1) if out.shape[i] > 1)
-    reach = V
-    for stride, n in dims:
-        _need(stride >= reach, "out: its rows overlap")
+        return torch.empty_like(logits)          # rows of the same alignment as those of the logits where they are dense
+    if out is logits and logits.is_contiguous():
+        return out
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out: the logits' shape, type and device")
+    if out.stride(-1) != 1 and out.shape[-1] != 1:
+        raise ValueError("out: the last dimension has to be dense")
+    reach = out.shape[-1]
+    for stride, n in sorted((out.stride(i), out.shape[i]) for i in range(out.dim() - 1) if out.shape[i] > 1):
+        if stride < reach:
+            raise ValueError("out: its rows overlap")
         reach = stride * (n - 1) + reach
     if out.numel() and not (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()):
-        first, last = _span(out)
-        a, b = _span(logits)
-        _need(last <= a or b <= first, "out: overlaps the logits without being them")
+        (first, last), (a, b) = _span(out), _span(logits)
+        if not (last <= a or b <= first):
+            raise ValueError("out: overlaps the logits without being them")
     return out
 
 
@@ -128,30 +126,37 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))
 
 
+_status = {}            # device index -> address of its status word
+
+
 def _rows(logits, grad=None):
-    two = logits.dim() == 2
-    S = logits.shape[0] if two else logits.shape[1]
-    T = logits.shape[:-1].numel()
-    strides = lambda t: (0, 0) if t is None else ((0, t.stride(0)) if two else (t.stride(0), t.stride(1)))
-    zb, zs = strides(logits)
-    db, ds = strides(grad)
-    return _Rows(logits.data_ptr(), ptr(grad), zb, zs, db, ds, T, max(S, 1), logits.shape[-1], int(logits.dtype == torch.float32),
-                 _lib.status_word(logits.device).data_ptr())
+    st, sh, dev = logits.stride(), logits.shape, logits.device.index
+    status = _status.get(dev)
+    if status is None:
+        status = _status[dev] = _lib.status_word(logits.device).data_ptr()
+    d, dz = ((0, 0, 0), 0) if grad is None else (grad.stride(), grad.data_ptr())
+    f32 = logits.dtype is torch.float32
+    if len(sh) == 2:
+        return _ROWS.pack(logits.data_ptr(), dz, 0, st[0], 0, d[0], sh[0], max(sh[0], 1), sh[1], f32, status)
+    return _ROWS.pack(logits.data_ptr(), dz, st[0], st[1], d[0], d[1], sh[0] * sh[1], max(sh[1], 1), sh[2], f32, status)
 
 
-def _on(device):
-    """The device of the tensors, current for the launch: streams and kernels belong to the device that is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _call(device, what, launches, fn, *args):
+    """fn(*args, stream) with the tensors' device current: streams and kernels belong to the device that is."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what, launches)
+        return
+    with torch.cuda.device(index):
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what, launches)
 
 
 def _empty(device, *sizes, dtype=torch.float32):
     return torch.empty(sizes, dtype=dtype, device=device)
 
 
-def _zero_(grad):
-    return grad.zero_() if grad is not None else None
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _softmax64(z):
@@ -193,15 +198,10 @@ def logprobs_fwd(logits, targets, ignore_index: int = -100):
         keep, _, lp, (_, m, ls) = _taken(logits, targets, ignore_index)
         return lp.float(), torch.where(keep, torch.stack([m, ls]), torch.zeros((), dtype=m.dtype)).float()
     lp, stats = _empty(logits.device, *targets.shape), _empty(logits.device, 2, *targets.shape)
-    _score_rows(logits, targets, ignore_index, lp, None, stats)
-    return lp, stats
-
-
-def _score_rows(logits, targets, ignore_index, lp, lse, stats):
     if targets.numel():
-        with _on(logits.device):
-            check(_lib.lib().tfb_token_logprobs(_rows(logits), targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), ptr(lp), ptr(lse),
-                                                ptr(stats), stream()), "token_logprobs")
+        _call(logits.device, "token_logprobs", 1, _lib.lib().tfb_token_logprobs, _rows(logits), targets.data_ptr(), targets.dtype is torch.int64, int(ignore_index),
+              lp.data_ptr(), stats.data_ptr())
+    return lp, stats
 
 
 def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=None):
@@ -209,7 +209,7 @@ def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=No
     _check_logits(logits)
     targets = _check_index(targets, logits.shape[:-1], "targets", logits.device)
     dlogp = _check_f32(dlogp, targets.shape, "dlogp", logits.device)
-    stats = _check_f32(stats, (2, *targets.shape), "stats", logits.device)
+    stats = _check_f32(stats, torch.Size((2, *targets.shape)), "stats", logits.device)
     grad = _gradient(logits, out, True)
     if not logits.is_cuda:
         keep, y, lp, soft = _taken(logits, targets, ignore_index)
@@ -217,9 +217,8 @@ def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=No
         _row_gradient(y, c, soft, keep, grad)
         return grad
     if targets.numel():
-        with _on(logits.device):
-            check(_lib.lib().tfb_token_logprobs_bwd(_rows(logits, grad), targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index),
-                                                    stats.data_ptr(), dlogp.data_ptr(), stream()), "token_logprobs_bwd")
+        _call(logits.device, "token_logprobs_bwd", 1, _lib.lib().tfb_token_logprobs_bwd, _rows(logits, grad), targets.data_ptr(), targets.dtype is torch.int64,
+              int(ignore_index), stats.data_ptr(), dlogp.data_ptr())
     return grad
 
 
@@ -268,16 +267,18 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     _check_logits(logits)
     dev = logits.device
     targets = _check_index(targets, logits.shape[:-1], "targets", dev)
-    _need(kl in _KL, f"kl: one of {sorted(_KL)}, got {kl!r}")
-    _need(mean in _MEAN, f"mean: one of {sorted(_MEAN)}, got {mean!r}")
-    _need(mean == "tokens" or n_valid is None, "n_valid: belongs to the mean over tokens")
-    _need(kl_coef == 0.0 or ref_logprobs is not None, "kl_coef: wants reference log-probabilities")
+    kl_kind, mean_kind = _one_of(kl, _KL, "kl"), _one_of(mean, _MEAN, "mean")
+    if n_valid is not None and mean != "tokens":
+        raise ValueError("n_valid: belongs to the mean over tokens")
+    if kl_coef != 0.0 and ref_logprobs is None:
+        raise ValueError("kl_coef: wants reference log-probabilities")
     adv_seq = logits.dim() == 3 and advantages.dim() == 1
     advantages = _check_f32(advantages, targets.shape[:1] if adv_seq else targets.shape, "advantages", dev)
     old, ref = _check_f32(old_logprobs, targets.shape, "old_logprobs", dev), _check_f32(ref_logprobs, targets.shape, "ref_logprobs", dev)
     n_valid = _check_n_valid(n_valid, dev)
     lo, hi = (math.inf, math.inf) if clip is None else (float(clip[0]), float(clip[1])) if isinstance(clip, (tuple, list)) else (float(clip), float(clip))
-    _need(lo >= 0 and hi >= 0, f"clip: bounds of 0 or more, got {clip!r}")
+    if not (lo >= 0 and hi >= 0):
+        raise ValueError(f"clip: bounds of 0 or more, got {clip!r}")
     ratio = old is not None or clip is not None
     grad = _gradient(logits, out, want_grad)
     B, S = targets.shape if targets.dim() == 2 else (1, targets.shape[0])
@@ -316,12 +317,10 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     n_ws = max(3 * T, 6 * min(T, PIPE_CLUSTERS))
     sums, work = _empty(dev, 3), _empty(dev, n_ws + B + 1)
     ws = work.data_ptr()
-    arg = _Policy(targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), advantages.data_ptr(), ptr(old), ptr(ref), int(adv_seq), int(ratio),
-                  _KL[kl], _MEAN[mean], 1 - lo, 1 + hi, float(kl_coef), ptr(n_valid), lp.data_ptr(), sums.data_ptr(),
-                  ws, ws + 4 * n_ws, ws + 4 * (n_ws + B))
-    with _on(dev):
-        check(_lib.lib().tfb_policy_loss(_rows(logits, grad), arg, stream()), "policy_loss", 2)
-    return PolicyLoss(sums[0], sums[1], sums[2], lp, grad)
+    arg = _POLICY.pack(targets.data_ptr(), targets.dtype is torch.int64, int(ignore_index), advantages.data_ptr(), _at(old), _at(ref), adv_seq, ratio, kl_kind, mean_kind,
+                       1 - lo, 1 + hi, float(kl_coef), _at(n_valid), lp.data_ptr(), sums.data_ptr(), ws, ws + 4 * n_ws, ws + 4 * (n_ws + B))
+    _call(dev, "policy_loss", 2, _lib.lib().tfb_policy_loss, _rows(logits, grad), arg)
+    return PolicyLoss(*sums.unbind(), lp, grad)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -344,14 +343,16 @@ def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float =
     with e = ``label_smoothing``, "hinge" max(0, 1 - beta h), "squared" (h - 1 / (2 beta))^2."""
     _check_logits(logits)
     dev = logits.device
-    _need(logits.dim() == 3 and logits.shape[0] % 2 == 0, f"logits: [2N, S, V], got {tuple(logits.shape)}")
+    if logits.dim() != 3 or logits.shape[0] % 2:
+        raise ValueError(f"logits: [2N, S, V], got {tuple(logits.shape)}")
     targets = _check_index(targets, logits.shape[:-1], "targets", dev)
-    _need(kind in _KIND, f"kind: one of {sorted(_KIND)}, got {kind!r}")
-    _need(beta > 0, f"beta: more than 0, got {beta}")
-    _need(0 <= label_smoothing < 0.5, f"label_smoothing: in [0, 0.5), got {label_smoothing}")
-    _need(label_smoothing == 0 or kind == "sigmoid", "label_smoothing: belongs to the sigmoid loss")
+    loss_kind = _one_of(kind, _KIND, "kind")
+    if not 0 < beta < math.inf:
+        raise ValueError(f"beta: more than 0, got {beta}")
+    if not 0 <= label_smoothing < 0.5 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError(f"label_smoothing: in [0, 0.5), of the sigmoid loss, got {label_smoothing} ({kind})")
     N, S = logits.shape[0] // 2, logits.shape[1]
-    ref = _check_f32(ref_logprobs, (2 * N,), "ref_logprobs", dev)
+    ref = _check_f32(ref_logprobs, torch.Size((2 * N,)), "ref_logprobs", dev)
     grad = _gradient(logits, out, want_grad)
     if not logits.is_cuda:
         keep, y, lp, soft = _taken(logits, targets, ignore_index)
@@ -380,13 +381,12 @@ def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float =
         l = {"sigmoid": torch.nn.functional.softplus(-x) + label_smoothing * x, "hinge": (1 - x).clamp(min=0), "squared": (x / beta - 0.5 / beta) ** 2}[kind]
         return PreferenceLoss(l.sum() / max(N, 1), x, L, grad)
     T = 2 * N * S
-    loss, lp64, work = _empty(dev, 1), _empty(dev, T, dtype=torch.float64), _empty(dev, 2 * T + 3 * N + 1)
-    arg = _Preference(targets.data_ptr(), int(targets.dtype == torch.int64), int(ignore_index), ptr(ref), _KIND[kind], int(average), float(beta),
-                      float(label_smoothing), loss.data_ptr(), margins.data_ptr(), L.data_ptr(), lp64.data_ptr(), work.data_ptr(),
-                      work.data_ptr() + 8 * T, work.data_ptr() + 8 * T + 8 * N, work.data_ptr() + 8 * T + 12 * N)
-    with _on(dev):
-        check(_lib.lib().tfb_preference_loss(_rows(logits, grad), arg, stream()), "preference_loss", 3 if want_grad else 2)
-    return PreferenceLoss(loss[0], margins, L, grad)
+    loss, lp64, work = _empty(dev), _empty(dev, T, dtype=torch.float64), _empty(dev, 2 * T + 3 * N + 1)
+    ws = work.data_ptr()
+    arg = _PREFERENCE.pack(targets.data_ptr(), targets.dtype is torch.int64, int(ignore_index), _at(ref), loss_kind, bool(average), float(beta), float(label_smoothing),
+                           loss.data_ptr(), margins.data_ptr(), L.data_ptr(), lp64.data_ptr(), ws, ws + 8 * T, ws + 8 * T + 8 * N, ws + 8 * T + 12 * N)
+    _call(dev, "preference_loss", 3 if want_grad else 2, _lib.lib().tfb_preference_loss, _rows(logits, grad), arg)
+    return PreferenceLoss(loss, margins, L, grad)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -409,14 +409,15 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     the number of rows with entries."""
     _check_logits(logits)
     dev, V = logits.device, logits.shape[-1]
-    _need(top_ids.dim() == logits.dim() and top_ids.shape[-1] >= 1, f"top_ids: {tuple(logits.shape[:-1])} + [K] wanted, got {tuple(top_ids.shape)}")
+    if top_ids.dim() != logits.dim() or top_ids.shape[-1] < 1 or top_ids.shape[-1] > MAX_TOP:
+        raise ValueError(f"top_ids: {tuple(logits.shape[:-1])} + [K] wanted, K up to {MAX_TOP}, got {tuple(top_ids.shape)}")
     K = top_ids.shape[-1]
-    _need(K <= MAX_TOP, f"top_ids: up to {MAX_TOP} entries a row, got {K}")
-    top_ids = _check_index(top_ids, (*logits.shape[:-1], K), "top_ids", dev)
-    _need(top_logits.shape == top_ids.shape and top_logits.device == dev, f"top_logits: {tuple(top_ids.shape)} on {dev} wanted, got {tuple(top_logits.shape)} on {top_logits.device}")
-    _need(top_logits.dtype in (torch.bfloat16, torch.float32), f"top_logits: bfloat16 or float32, got {top_logits.dtype}")
+    top_ids = _check_index(top_ids, torch.Size((*logits.shape[:-1], K)), "top_ids", dev)
+    if top_logits.shape != top_ids.shape or top_logits.device != dev or top_logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"top_logits: bfloat16 or float32 {tuple(top_ids.shape)} on {dev} wanted, got {top_logits.dtype} {tuple(top_logits.shape)} on {top_logits.device}")
     top_logits = top_logits.contiguous()
-    _need(temperature > 0 and math.isfinite(temperature), f"temperature: more than 0, got {temperature}")
+    if not 0 < temperature < math.inf:
+        raise ValueError(f"temperature: more than 0, got {temperature}")
     n_valid = _check_n_valid(n_valid, dev)
     grad = _gradient(logits, out, want_grad)
     rows = logits.shape[:-1]
@@ -443,44 +444,62 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     if not T:
         return DistillLoss(torch.zeros((), device=dev), kl, grad)
     n_ws = max(T, 6 * min(T, PIPE_CLUSTERS))
-    loss, work = _empty(dev, 1), _empty(dev, n_ws + 2)
+    loss, work = _empty(dev), _empty(dev, n_ws + 2)
     ws = work.data_ptr()
-    arg = _Distill(top_ids.data_ptr(), top_logits.data_ptr(), int(top_ids.dtype == torch.int64), int(top_logits.dtype == torch.float32), K, float(temperature),
-                   ptr(n_valid), kl.data_ptr(), loss.data_ptr(), ws, ws + 4 * n_ws, ws + 4 * n_ws + 4)
-    with _on(dev):
-        check(_lib.lib().tfb_distill_loss(_rows(logits, grad), arg, stream()), "distill_loss", 2)
-    return DistillLoss(loss[0], kl, grad)
+    arg = _DISTILL.pack(top_ids.data_ptr(), top_logits.data_ptr(), top_ids.dtype is torch.int64, top_logits.dtype is torch.float32, K, float(temperature), _at(n_valid),
+                        kl.data_ptr(), loss.data_ptr(), ws, ws + 4 * n_ws, ws + 4 * n_ws + 4)
+    _call(dev, "distill_loss", 2, _lib.lib().tfb_distill_loss, _rows(logits, grad), arg)
+    return DistillLoss(loss, kl, grad)
 
 
 # ---------------------------------------------------------------------------------------------
 # scoring from hidden states
 # ---------------------------------------------------------------------------------------------
-SCORE_CHUNK = 1 << 28          # logits that exist at a time
+SCORE_ROWS = 1 << 15          # rows of one launch: bounds its workspace (a row's hidden state, and 8 bytes per 128 of the vocabulary)
+
+
+def _tma_ready(t):
+    """Rows that start at 16-byte boundaries."""
+    if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def linear_logprobs(x, weight, targets, ignore_index: int = -100):
     """Log-probabilities of given tokens under a head, and the logsumexp of its logits, without all of the logits in memory: x [..., H], weight [V, H] (bfloat16, or
     float32 on the CPU), targets of x's leading shape -> (logp, lse), float32, both 0 where the target is ``ignore_index``.  For passes that want
     no gradient (reference models, older policies, evaluation); with one use ``token_logprobs`` on the logits."""
-    _need(not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)), "linear_logprobs has no gradient: call it under torch.no_grad(), or use token_logprobs")
-    _need(x.dim() >= 1 and weight.dim() == 2 and weight.shape[1] == x.shape[-1], f"x [..., H] and weight [V, H], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    _need(x.dtype == weight.dtype, f"x and weight: one type, got {x.dtype} and {weight.dtype}")
-    _need(x.device == weight.device, f"weight: on {weight.device}, x is on {x.device}")
-    _need(weight.shape[0] > 0 and weight.shape[1] > 0, "an empty weight")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        raise ValueError("linear_logprobs has no gradient: call it under torch.no_grad(), or use token_logprobs")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.numel() == 0:
+        raise ValueError(f"x [..., H] and weight [V, H], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dtype != weight.dtype or x.device != weight.device:
+        raise ValueError(f"x and weight: one type and device, got {x.dtype} on {x.device} and {weight.dtype} on {weight.device}")
     targets = _check_index(targets, x.shape[:-1], "targets", x.device)
-    x2, y = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
+    x2, y = x.reshape(-1, x.shape[-1]), targets.view(-1)
     if not x.is_cuda:
-        _need(x.is_floating_point(), f"x: a floating type, got {x.dtype}")
+        if not x.is_floating_point():
+            raise ValueError(f"x: a floating type, got {x.dtype}")
         keep, _, lp, (_, m, ls) = _taken(x2.float() @ weight.float().t(), y, ignore_index)
         return lp.float().view(targets.shape), torch.where(keep, m + ls, torch.zeros((), dtype=m.dtype)).float().view(targets.shape)
-    _need(x.dtype == torch.bfloat16, f"x: bfloat16 on the GPU, got {x.dtype}")
-    _need(x.shape[-1] % 8 == 0, f"x: a width that is a multiple of 8, got {x.shape[-1]}")
-    ready = lambda t: t if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-    x2, w = ready(x2), ready(weight)
-    lp, lse = _empty(x.device, y.numel()), _empty(x.device, y.numel())
-    with _on(x.device):
-        step = max(1, SCORE_CHUNK // w.shape[0])
-        for a in range(0, y.numel(), step):
-            part = slice(a, a + step)
-            _score_rows(F.gemm(x2[part], w, out_dtype=torch.float32), y[part], ignore_index, lp[part], lse[part], None)
-    return lp.view(targets.shape), lse.view(targets.shape)
+    if x.dtype is not torch.bfloat16 or x.shape[-1] % 8:
+        raise ValueError(f"x: bfloat16 of a width that is a multiple of 8 on the GPU, got {x.dtype} {tuple(x.shape)}")
+    x2, w, dev = _tma_ready(x2), _tma_ready(weight), x.device
+    lp, lse = _empty(dev, *targets.shape), _empty(dev, *targets.shape)
+    (V, H), M = w.shape, y.numel()
+    if not M:
+        return lp, lse
+    n = min(M, SCORE_ROWS)
+    # workspace: parts of a row's statistics (two values per half a tile), compacted rows and their number; the logits of few rows
+    ldz = -(-V // 4) * 4 if n <= 128 and n * V <= 1 << 27 else 0
+    parts = 4 * -(-V // (128 if n <= 128 else 256)) * n
+    xc, work = _empty(dev, n, H, dtype=torch.bfloat16), _empty(dev, parts + ldz * n + 3 * n + 1)
+    ws = work.data_ptr()
+    stats, rows = ws + 4 * (parts + ldz * n), ws + 4 * (parts + ldz * n + 2 * n)
+    status = _lib.status_word(dev).data_ptr()
+    for a in range(0, M, n):
+        arg = _SCORE.pack(x2.data_ptr() + 2 * a * x2.stride(0), w.data_ptr(), x2.stride(0), w.stride(0), y.data_ptr() + y.element_size() * a, y.dtype is torch.int64,
+                          int(ignore_index), min(n, M - a), V, H, lp.data_ptr() + 4 * a, lse.data_ptr() + 4 * a, rows, rows + 4, xc.data_ptr(), H, ws, 0,
+                          ws + 4 * parts if ldz else 0, ldz, stats)
+        _call(dev, "linear_logprobs", 3, _lib.lib().tfb_linear_logprobs, arg, status)
+    return lp, lse
