@@ -96,6 +96,22 @@ __device__ __forceinline__ void block_join(float& m, float& s, float k, float2* 
   s = __shfl_sync(~0u, s, 0);
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+// (m, s) of all lanes together, the same bits in every lane
+__device__ __forceinline__ void warp_join(float& m, float& s, float k) {
+  const float M = warp_max(m), r = M == -INFINITY ? 0.f : M;
+  s = warp_sum(s * ex2((m - r) * k));
+  m = M;
+}
 // log s to a few 1e-8 (absolute), where logf(s) alone has the rounding of its result: the exponent's part in 64 bits, the rest in [0, log 2)
 __device__ __forceinline__ double log64(float s) {
   if (!(s >= 1.f && s < INFINITY)) return double(logf(s));
@@ -222,14 +238,15 @@ __device__ __forceinline__ void batch_stats(const float (&f)[U][N], float k, flo
   m = mx;
 }
 
+// tid, nt: thread of those that share the row, and how many they are
 template <class T, int U>
-__device__ __forceinline__ void row_stats(const T* row, int V, float k, float& m, float& s) {
+__device__ __forceinline__ void row_stats(const T* row, int V, float k, float& m, float& s, int tid, int nt) {
   constexpr int N = Vec<T>::N;
   m = -INFINITY;
   s = 0.f;
-  const int head = head_of(row, V), nv = (V - head) / N, nt = blockDim.x;
+  const int head = head_of(row, V), nv = (V - head) / N;
   const uint4* v = reinterpret_cast<const uint4*>(row + head);
-  int i = threadIdx.x;
+  int i = tid;
   for (; i + (U - 1) * nt < nv; i += U * nt) {
     uint4 w[U];
     float f[U][N];
@@ -245,22 +262,22 @@ __device__ __forceinline__ void row_stats(const T* row, int V, float k, float& m
     batch_stats<1, N>(f, k, m, s);
   }
   const int tail = head + nv * N;
-  if (int(threadIdx.x) < head) join(m, s, Vec<T>::get(row[threadIdx.x]), 1.f, k);
-  if (tail + int(threadIdx.x) < V) join(m, s, Vec<T>::get(row[tail + threadIdx.x]), 1.f, k);
+  if (tid < head) join(m, s, Vec<T>::get(row[tid]), 1.f, k);
+  if (tail + tid < V) join(m, s, Vec<T>::get(row[tail + tid]), 1.f, k);
 }
 
 template <class T>
-__device__ __forceinline__ void row_zero(T* row, int V) {
+__device__ __forceinline__ void row_zero(T* row, int V, int tid, int nt) {
   constexpr int N = Vec<T>::N;
   const int head = head_of(row, V), nv = (V - head) / N, tail = head + nv * N;
-  for (int i = threadIdx.x; i < nv; i += blockDim.x) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
-  if (int(threadIdx.x) < head) row[threadIdx.x] = Vec<T>::put(0.f);
-  if (tail + int(threadIdx.x) < V) row[tail + threadIdx.x] = Vec<T>::put(0.f);
+  for (int i = tid; i < nv; i += nt) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
+  if (tid < head) row[tid] = Vec<T>::put(0.f);
+  if (tail + tid < V) row[tail + tid] = Vec<T>::put(0.f);
 }
 
 // dz = c exp2((z - m) k), minus hot at index y
 template <class T>
-__device__ __forceinline__ void row_grad(const T* row, T* out, int V, float k, float m, float c, long long y, float hot) {
+__device__ __forceinline__ void row_grad(const T* row, T* out, int V, float k, float m, float c, long long y, float hot, int tid, int nt) {
   constexpr int N = Vec<T>::N;
   const int head = head_of(row, V), nv = (V - head) / N, tail = head + nv * N;
   const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
@@ -270,7 +287,7 @@ __device__ __forceinline__ void row_grad(const T* row, T* out, int V, float k, f
     if (i == y) g -= hot;
     out[i] = Vec<T>::put(g);
   };
-  for (int i = threadIdx.x; i < nv; i += blockDim.x) {
+  for (int i = tid; i < nv; i += nt) {
     float f[N];
     Vec<T>::unpack(v[i], f);
 #pragma unroll
@@ -285,19 +302,26 @@ __device__ __forceinline__ void row_grad(const T* row, T* out, int V, float k, f
       for (int j = 0; j < N; ++j) out[head + i * N + j] = Vec<T>::put(f[j]);
     }
   }
-  if (int(threadIdx.x) < head) one(threadIdx.x);
-  if (tail + int(threadIdx.x) < V) one(tail + threadIdx.x);
+  if (tid < head) one(tid);
+  if (tail + tid < V) one(tail + tid);
 }
 
-constexpr int ROW_THREADS = 512;
+constexpr int ROW_THREADS = 512, WARP_ROWS = 8, WARP_TOP = 128;      // rows of a block, and most entries of a teacher's, with a warp to a row
 
-template <class T, int MODE>
-__global__ void __launch_bounds__(ROW_THREADS, 4) row_loss_kernel(const RowsArg r, const LossArg a) {
+// WARP: a warp to a row, WARP_ROWS rows to a block; else a block to a row.
+template <class T, int MODE, bool WARP>
+__global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 : MODE == MODE_GRAD ? 4 : 3) row_loss_kernel(const RowsArg r, const LossArg a) {
   tfb::pdl_sync();
   __shared__ float2 sh[32];
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : int(blockDim.x), warp = threadIdx.x >> 5;
+  auto sync = [&] { if constexpr (WARP) __syncwarp(); else __syncthreads(); };
+  auto join_all = [&](float& m, float& s, float k) { if constexpr (WARP) warp_join(m, s, k); else block_join(m, s, k, sh); };
   extern __shared__ __align__(128) char dyn[];         // MODE_DISTILL: K teacher weights, K ids
   if (a.zero && blockIdx.x == 0 && threadIdx.x == 0) *a.zero = 0;
-  const long long t = blockIdx.x, b = t / r.S, pos = t - b * r.S;
+  // the gradient of given statistics goes from the last row to the first: the pass that took them has left the last ones in L2
+  const long long place = MODE == MODE_GRAD ? gridDim.x - 1 - blockIdx.x : blockIdx.x, t = WARP ? place * WARP_ROWS + warp : place;
+  if (WARP && t >= r.T) return;
+  const long long b = t / r.S, pos = t - b * r.S;
   const T* row = static_cast<const T*>(r.z) + b * r.zb + pos * r.zs;
   T* out = r.dz ? static_cast<T*>(r.dz) + b * r.db + pos * r.ds : nullptr;
   const float k = MODE == MODE_DISTILL ? LOG2E * a.inv_tau : LOG2E;
@@ -305,19 +329,19 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) row_loss_kernel(const RowsArg 
   if constexpr (MODE == MODE_DISTILL) {
     const bool off = ld_idx(a.top_ids, t * a.K, a.idx64) < 0;
     if (off) {
-      if (threadIdx.x == 0) { a.logp[t] = 0.f; a.terms[t] = 0.f; }
-      if (out) row_zero(out, r.V);
+      if (tid == 0) { a.logp[t] = 0.f; a.terms[t] = 0.f; }
+      if (out) row_zero(out, r.V, tid, nt);
       return;
     }
-    float* q = reinterpret_cast<float*>(dyn);
+    float* q = reinterpret_cast<float*>(dyn) + (WARP ? warp * 2 * a.K : 0);
     int* id = reinterpret_cast<int*>(q + a.K);
     float m, s;
-    row_stats<T, 2>(row, r.V, k, m, s);
-    block_join(m, s, k, sh);
-    __syncthreads();
+    row_stats<T, 2>(row, r.V, k, m, s, tid, nt);
+    join_all(m, s, k);
+    sync();
     // the teacher's weights: soft-max over the row's entries
     float tm = -INFINITY, ts = 0.f;
-    for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
+    for (int j = tid; j < a.K; j += nt) {
       const long long y = ld_idx(a.top_ids, t * a.K + j, a.idx64);
       TFB_BOUNDS(y < r.V, 3, y, r.V);
       const bool have = y >= 0 && y < r.V;
@@ -326,26 +350,31 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) row_loss_kernel(const RowsArg 
       id[j] = y >= r.V ? -2 : (have ? int(y) : -1);
       join(tm, ts, z, 1.f, k);
     }
-    block_join(tm, ts, k, sh);
+    join_all(tm, ts, k);
     const float tr = tm == -INFINITY ? 0.f : tm;
     float kl = 0.f;
     bool bad = false;
     const float mr = m == -INFINITY ? 0.f : m, ls = logf(s), lts = logf(ts);
-    for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
+    for (int j = tid; j < a.K; j += nt) {
       if (id[j] == -2) bad = true;
       const float lq = (q[j] - tr) * a.inv_tau - lts, w = ex2((q[j] - tr) * k) / ts;
       q[j] = id[j] >= 0 ? w : 0.f;
       if (id[j] >= 0 && q[j] != 0.f) kl += q[j] * (lq - ((Vec<T>::get(row[id[j]]) - mr) * a.inv_tau - ls));
     }
-    const int any_bad = __syncthreads_or(bad);
+    int any_bad;
+    if constexpr (WARP) { any_bad = __any_sync(~0u, bad); __syncwarp(); } else any_bad = __syncthreads_or(bad);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) kl += __shfl_xor_sync(~0u, kl, o);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5].x = kl;
-    __syncthreads();
+    if constexpr (!WARP) {
+      if ((threadIdx.x & 31) == 0) sh[warp].x = kl;
+      __syncthreads();
+    }
     const float w = any_bad ? NAN : weight_of(a, t, r.S);
-    if (threadIdx.x == 0) {
-      kl = 0.f;
-      for (int i = 0; i < int(blockDim.x >> 5); ++i) kl += sh[i].x;
+    if (tid == 0) {
+      if constexpr (!WARP) {
+        kl = 0.f;
+        for (int i = 0; i < ROW_THREADS / 32; ++i) kl += sh[i].x;
+      }
       if (any_bad) kl = NAN;
       a.logp[t] = kl;
       a.terms[t] = kl * a.tau * a.tau * w;
@@ -353,11 +382,11 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) row_loss_kernel(const RowsArg 
     if (!out) return;
     // the entries' own gradients, each from its value of z, before the row is written (it may be written in place)
     const float c = a.tau * w;
-    constexpr int PER = TL_MAX_TOP / ROW_THREADS;
+    constexpr int PER = WARP ? WARP_TOP / 32 : TL_MAX_TOP / ROW_THREADS;
     float g[PER];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int j = threadIdx.x + u * ROW_THREADS;
+      const int j = tid + u * nt;
       g[u] = 0.f;
       if (j < a.K && id[j] >= 0) {
         float sum = 0.f;
@@ -365,43 +394,43 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) row_loss_kernel(const RowsArg 
         g[u] = c * (ex2((Vec<T>::get(row[id[j]]) - mr) * k) / s - sum);
       }
     }
-    __syncthreads();
-    row_grad(row, out, r.V, k, mr, c / s, -1, 0.f);
-    __syncthreads();
+    sync();
+    row_grad(row, out, r.V, k, mr, c / s, -1, 0.f, tid, nt);
+    sync();
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int j = threadIdx.x + u * ROW_THREADS;
+      const int j = tid + u * nt;
       if (j < a.K && id[j] >= 0) out[id[j]] = Vec<T>::put(g[u]);
     }
     return;
   } else {
     const long long y = ld_idx(a.targets, t, a.idx64);
     if (y == a.ignore) {
-      if (threadIdx.x == 0) {
+      if (tid == 0) {
         put_stats<MODE>(a, r.T, t, 0.f, 0.0, 0.0);
         if (MODE == MODE_POLICY) a.terms[t] = a.terms[r.T + t] = a.terms[2ll * r.T + t] = 0.f;
       }
-      if (MODE != MODE_STATS && out) row_zero(out, r.V);
+      if (MODE != MODE_STATS && out) row_zero(out, r.V, tid, nt);
       return;
     }
-    if (threadIdx.x == 0) TFB_BOUNDS(y >= 0 && y < r.V, 3, y, r.V);
+    if (tid == 0) TFB_BOUNDS(y >= 0 && y < r.V, 3, y, r.V);
     const float zy = y >= 0 && y < r.V ? Vec<T>::get(row[y]) : NAN;       // a target outside the vocabulary makes its row NaN
     if constexpr (MODE == MODE_GRAD) {
       const float m = a.stats[t], mr = m == -INFINITY ? 0.f : m, p = ex2(-a.stats[r.T + t] * k);       // 1 / S
       const float c = zy != zy ? NAN : (a.per_seq ? a.dlogp[b] : a.dlogp[t]);
-      __syncthreads();
-      row_grad(row, out, r.V, k, mr, -c * p, y, -c);
+      sync();
+      row_grad(row, out, r.V, k, mr, -c * p, y, -c, tid, nt);
     } else {
       float m, s;
-      row_stats<T, 2>(row, r.V, k, m, s);
-      block_join(m, s, k, sh);
+      row_stats<T, 2>(row, r.V, k, m, s, tid, nt);
+      join_all(m, s, k);
       const double ls = log64(s), lp64 = double(zy) - double(m) - ls;
       float g = 0.f, w = 0.f, l = 0.f, kl = 0.f, clipped = 0.f;
       if constexpr (MODE == MODE_POLICY) {
         w = weight_of(a, t, r.S);
         policy_row(a, lp64, t, b, l, kl, clipped, g);
       }
-      if (threadIdx.x == 0) {
+      if (tid == 0) {
         put_stats<MODE>(a, r.T, t, m, ls, lp64);
         if constexpr (MODE == MODE_POLICY) {
           a.terms[t] = w * l;
@@ -411,7 +440,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) row_loss_kernel(const RowsArg 
       }
       if (MODE == MODE_POLICY && out) {
         const float c = w * g;
-        row_grad(row, out, r.V, k, m == -INFINITY ? 0.f : m, -c / s, y, -c);
+        sync();                        // everyone has read the target's logit (the row may be written in place)
+        row_grad(row, out, r.V, k, m == -INFINITY ? 0.f : m, -c / s, y, -c, tid, nt);
       }
     }
   }
@@ -452,22 +482,6 @@ struct PipeArg {
   float* out;                          // [nsums]
 };
 
-__device__ __forceinline__ float warp_max(float v) {
-  float m;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-  return m;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
-}
-// (m, s) of all lanes together, the same bits in every lane
-__device__ __forceinline__ void warp_join(float& m, float& s, float k) {
-  const float M = warp_max(m), r = M == -INFINITY ? 0.f : M;
-  s = warp_sum(s * ex2((m - r) * k));
-  m = M;
-}
 __device__ __forceinline__ void st_async_v4(uint32_t addr, uint32_t bar, float4 v) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%2, %3, %4, %5}, [%1];" ::"r"(addr), "r"(bar), "f"(v.x), "f"(v.y), "f"(v.z),
                "f"(v.w)
@@ -960,7 +974,8 @@ __global__ void __launch_bounds__(1024) row_count_kernel(const void* idx, int id
     return;
   }
   int c = 0;
-  for (long long t = threadIdx.x; t < (long long)N * S; t += 1024) c += counts(t);
+#pragma unroll 8
+  for (int t = threadIdx.x; t < N * S; t += 1024) c += counts(t);
   c = __reduce_add_sync(~0u, c);
   if (lane == 0) sh[warp] = c;
   __syncthreads();
@@ -983,16 +998,30 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
   return v;
 }
 
-// out[i] = sum of terms[i * T ...], i < n, in 64 bits and always in the same order
-__global__ void __launch_bounds__(1024) term_sum_kernel(const float* terms, int T, int n, float* out) {
+// out[i] = sum of terms[i * T ...], i < n <= 3, in 64 bits and always in the same order: every block a share of the rows, the block that ends last the shares.
+constexpr int TERM_BLOCKS = 32;
+__global__ void __launch_bounds__(512) term_sum_kernel(const float* terms, int T, int n, double* partial, int* counter, float* out) {
   tfb::pdl_sync();
   __shared__ double sh[32];
+  __shared__ int last;
+  const int share = (T + gridDim.x - 1) / gridDim.x, t0 = blockIdx.x * share, t1 = min(T, t0 + share);
   for (int i = 0; i < n; ++i) {
     double v = 0.0;
-    for (int t = threadIdx.x; t < T; t += 1024) v += double(terms[(long long)i * T + t]);
+#pragma unroll 4
+    for (int t = t0 + threadIdx.x; t < t1; t += 512) v += double(terms[(long long)i * T + t]);
     v = block_sum(v, sh);
-    if (threadIdx.x == 0) out[i] = float(v);
+    if (threadIdx.x == 0) partial[blockIdx.x * 3 + i] = v;
   }
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(counter, 1) == int(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!last || threadIdx.x >= n) return;
+  __threadfence();
+  double v = 0.0;
+  for (int b = 0; b < int(gridDim.x); ++b) v += __ldcg(partial + b * 3 + threadIdx.x);
+  out[threadIdx.x] = float(v);
 }
 
 // One block per pair: sums of both answers' log-probabilities, margin, loss, and the coefficient of each answer's rows.
@@ -1068,12 +1097,24 @@ __global__ void __launch_bounds__(256) pair_kernel(const PairArg a) {
 }
 
 // The general form's launch.
-template <int MODE>
-static int launch_rows(const RowsArg& r, const LossArg& a, cudaStream_t st) {
+template <class T, int MODE>
+static void launch_rows_t(const RowsArg& r, const LossArg& a, bool warp, cudaStream_t st) {
   const size_t smem = MODE == MODE_DISTILL ? size_t(a.K) * 8 : 0;
-  if (r.f32) tfb::launch_k_rows(r.T, row_loss_kernel<float, MODE>, r.T, ROW_THREADS, smem, st, r, a);
-  else tfb::launch_k_rows(r.T, row_loss_kernel<__nv_bfloat16, MODE>, r.T, ROW_THREADS, smem, st, r, a);
+  if (warp) tfb::launch_k_rows(r.T, row_loss_kernel<T, MODE, true>, (r.T + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, smem * WARP_ROWS, st, r, a);
+  else tfb::launch_k_rows(r.T, row_loss_kernel<T, MODE, false>, r.T, ROW_THREADS, smem, st, r, a);
+}
+template <int MODE>
+static int launch_rows(const RowsArg& r, const LossArg& a, bool warp, cudaStream_t st) {
+  if (r.f32) launch_rows_t<float, MODE>(r, a, warp, st);
+  else launch_rows_t<__nv_bfloat16, MODE>(r, a, warp, st);
   return int(cudaGetLastError());
+}
+
+// Rows for a warp each: the pipelined form takes 1.3 us for a row however short, per SM.  us of the policy loss, warps / that form: 50000 rows of 520 bytes 58 / 409, of 8 KB
+// 240 / 409, of 16 KB 509 / 424; 2000 rows of 520 bytes 10.9 / 26, of 8 KB 20 / 26, of 16 KB 30 / 27; 96 rows of 2 KB 8.5 / 9.6, of 4 KB 10.5 / 9.6, of 8 KB 13.3 / 9.9.
+static bool short_rows(const RowsArg& r, const LossArg& a) {
+  const long long bytes = r.V * (r.f32 ? 4ll : 2ll);
+  return a.K <= WARP_TOP && bytes <= (r.T >= 1024 ? 8192 : 2048);
 }
 
 // Clusters of `kern` that the device holds at a time (0: none; negative: -cudaError_t).  One entry per thread and kernel, since a run repeats its shapes.
@@ -1154,12 +1195,15 @@ template <int MODE>
 static int rows_and_sums(const RowsArg& r, LossArg a, int nsums, void* ws, int* counter, float* out, cudaStream_t st) {
   PipeArg q = {};
   q.nsums = nsums; q.partial = static_cast<double*>(ws); q.counter = counter; q.out = out;
-  int rc = launch_pipe<MODE>(r, a, q, st);
+  const bool warp = short_rows(r, a);
+  int rc = warp ? TFB_NOT_TAKEN : launch_pipe<MODE>(r, a, q, st);
   if (rc != TFB_NOT_TAKEN) return rc;
-  a.terms = static_cast<float*>(ws);
-  rc = launch_rows<MODE>(r, a, st);
+  a.terms = reinterpret_cast<float*>(static_cast<double*>(ws) + 3 * TERM_BLOCKS);
+  rc = launch_rows<MODE>(r, a, warp, st);
   if (rc || !nsums) return rc;
-  tfb::launch_k_rows(r.T, term_sum_kernel, 1, 1024, 0, st, static_cast<const float*>(ws), r.T, nsums, out);
+  double* partial = static_cast<double*>(ws);                     // in front of the terms
+  const int blocks = min(TERM_BLOCKS, (r.T + 2047) / 2048);
+  tfb::launch_k_rows(r.T, term_sum_kernel, blocks, 512, 0, st, a.terms, r.T, nsums, partial, counter, out);
   return int(cudaGetLastError());
 }
 
@@ -1194,7 +1238,7 @@ TFB_API int tfb_token_logprobs_bwd(const RowsArg* r, const void* targets, int id
   LossArg a = {};
   a.targets = targets; a.idx64 = idx64; a.ignore = ignore;
   a.stats = const_cast<float*>(stats); a.dlogp = dlogp;
-  return launch_rows<MODE_GRAD>(*r, a, static_cast<cudaStream_t>(stream));
+  return launch_rows<MODE_GRAD>(*r, a, short_rows(*r, a), static_cast<cudaStream_t>(stream));
 }
 
 struct PolicyArg {
@@ -1206,7 +1250,7 @@ struct PolicyArg {
   float lo, hi, kl_coef;
   const float* n_valid;                // 1 value: overrides the count of the mean over tokens
   float *logp, *out;                   // [T], [3]: loss, kl, share of clipped tokens
-  void* ws;                            // max(12 T, 24 min(T, PIPE_CLUSTERS)) bytes
+  void* ws;                            // 24 PIPE_CLUSTERS + 12 T bytes, aligned to 8
   float* denom;                        // workspace: [max(1, T / S)], and
   int* counter;                        // one word
 };
@@ -1256,7 +1300,7 @@ TFB_API int tfb_preference_loss(const RowsArg* r, const PreferenceArg* p, void* 
   tfb::launch_k_rows(r->T, pair_kernel, q.N, 256, 0, st, q);
   if (!r->dz) return int(cudaGetLastError());
   a.dlogp = p->coef; a.per_seq = 1; a.logp64 = nullptr; a.zero = nullptr;
-  return launch_rows<MODE_GRAD>(*r, a, st);
+  return launch_rows<MODE_GRAD>(*r, a, short_rows(*r, a), st);
 }
 
 struct DistillArg {
@@ -1265,7 +1309,7 @@ struct DistillArg {
   float tau;
   const float* n_valid;
   float *kl, *loss;                    // [T], [1]
-  void* ws;                            // max(4 T, 24 min(T, PIPE_CLUSTERS)) bytes
+  void* ws;                            // 24 PIPE_CLUSTERS + 4 T bytes, aligned to 8
   float* denom;                        // workspace: one value, and
   int* counter;                        // one word
 };

@@ -314,7 +314,7 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
         z = torch.zeros((), device=dev)
         return PolicyLoss(z, z, z, lp, grad)
     T = lp.numel()
-    n_ws = max(3 * T, 6 * min(T, PIPE_CLUSTERS))
+    n_ws = 6 * PIPE_CLUSTERS + 3 * T
     sums, work = _empty(dev, 3), _empty(dev, n_ws + B + 1)
     ws = work.data_ptr()
     arg = _POLICY.pack(targets.data_ptr(), targets.dtype is torch.int64, int(ignore_index), advantages.data_ptr(), _at(old), _at(ref), adv_seq, ratio, kl_kind, mean_kind,
@@ -443,7 +443,7 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     T = kl.numel()
     if not T:
         return DistillLoss(torch.zeros((), device=dev), kl, grad)
-    n_ws = max(T, 6 * min(T, PIPE_CLUSTERS))
+    n_ws = 6 * PIPE_CLUSTERS + T
     loss, work = _empty(dev), _empty(dev, n_ws + 2)
     ws = work.data_ptr()
     arg = _DISTILL.pack(top_ids.data_ptr(), top_logits.data_ptr(), top_ids.dtype is torch.int64, top_logits.dtype is torch.float32, K, float(temperature), _at(n_valid),
