@@ -1,0 +1,296 @@
+"""Trainers on the losses of ``ops/losses.py``: what one step does to the weights' gradients against plain autograd of the same formulas, the
+operators one after the other as a training run uses them, and scoring without logits.
+
+The gradients of a whole model are compared in fp32 on the CPU (two orders of the same 32-bit sums: 1e-5 of the largest entry), and on the GPU, where model and gradient are
+bfloat16, by the angle between them: every logit gradient is rounded to 2^-9 of itself in both, at different places, as are the products behind it."""
+import pytest
+import torch
+
+from transformers_fusion_b200.engines import dense as ED
+from transformers_fusion_b200.models.config import TransformerConfig
+from transformers_fusion_b200.models.dense import DenseModel
+from transformers_fusion_b200.ops import losses as L
+from transformers_fusion_b200.trainer import rl
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def model(dev, seed=0, V=96):
+    cfg = TransformerConfig(vocab_size=V, hidden_size=128, num_layers=2, num_heads=2, ffn_hidden_size=192, max_seq_len=64, init_std=0.1)
+    return DenseModel(cfg, device=dev, dtype=torch.float32 if dev == "cpu" else torch.bfloat16, seed=seed)
+
+
+def stepped_gradients(trainer, step):
+    """The flat gradient that a train_step hands to its optimizer, and what it returned."""
+    seen = {}
+
+    def take():
+        seen["g"] = trainer.flat.grads.clone()
+        trainer.flat.grads.zero_()
+    trainer.opt.step = take
+    out = step()
+    return seen["g"], out
+
+
+def plain_gradients(m, f):
+    m.flat.grads.zero_()
+    loss = f()
+    loss.backward()
+    for p in m.flat.params_list:
+        if p.grad is not None:
+            p.main_grad.add_(p.grad.float())
+            p.grad = None
+    g = m.flat.grads.clone()
+    m.flat.grads.zero_()
+    return g, float(loss.detach())
+
+
+def same(g, want, dev):
+    if dev == "cpu":
+        assert (g - want).abs().max() <= 1e-5 * want.abs().max()
+    else:
+        assert torch.nn.functional.cosine_similarity(g.double(), want.double(), dim=0) > 0.999
+        assert abs(g.norm() / want.norm() - 1) < 0.02
+
+
+def batch(dev, n=4, S=17, V=96, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, V, (n, S), generator=g)
+    mask = torch.zeros(n, S)
+    for i in range(n):
+        mask[i, 3 + i:S - i] = 1
+    return ids.to(dev), mask.to(dev), g
+
+
+def lp64(m, ids):
+    lp = torch.log_softmax(m(ids).float()[:, :-1], -1)
+    return lp.gather(-1, ids[:, 1:, None])[..., 0]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("clip,kl", [(0.0, 0.0), (0.2, 0.0), (0.0, 0.1), (0.2, 0.1)])
+def test_grpo_step(dev, clip, kl):
+    m = model(dev)
+    t = rl.GRPOTrainer(m, group_size=4, beta=0.04, clip_eps=clip, kl_coef=kl)
+    if kl:
+        t.ref_model = model(dev, seed=7).eval()
+    ids, mask, g = batch(dev)
+    rewards = torch.tensor([1.0, 0.2, -0.5, 0.7])
+    got, loss = stepped_gradients(t, lambda: t.train_step(ids, mask, rewards))
+    adv = t.advantages(rewards).to(dev)[:, None]
+
+    def plain():
+        lp, k = lp64(m, ids), mask[:, 1:]
+        n = k.sum(-1).clamp(min=1)
+        per = -torch.exp(lp - lp.detach()) * adv if clip else -adv * lp
+        out = ((per * k).sum(-1) / n).mean()
+        if kl:
+            with torch.no_grad():
+                r = lp64(t.ref_model, ids)
+            out = out + kl * (((torch.exp(r - lp) - (r - lp) - 1) * k).sum(-1) / n).mean()
+        return out
+    want, wloss = plain_gradients(m, plain)
+    same(got, want * (1 - 0.01 * 0.04), dev)
+    assert loss == pytest.approx(wloss, rel=1e-4, abs=1e-4)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("given", [False, True])
+def test_ppo_step(dev, given):
+    m = model(dev)
+    t = rl.PPOTrainer(m)
+    ids, mask, g = batch(dev)
+    old = None
+    if given:
+        with torch.no_grad():
+            old = lp64(m, ids) + 0.1 * torch.randn(4, 16, generator=g).to(dev)
+    seen = []
+    t.set_log_callback(lambda *a: seen.append(a))
+    real = t.values
+    coef = t.kl_coef
+    v = real(ids).detach()
+    got, (loss, vloss, kl) = stepped_gradients(t, lambda: t.train_step(ids, mask, torch.tensor([1.0, 0.0, -1.0, 0.5]), old))
+    k = mask[:, 1:]
+    advs = []
+    for b, r1 in enumerate([1.0, 0.0, -1.0, 0.5]):
+        r = torch.zeros(16)
+        r[int(k[b].nonzero().max())] = r1
+        advs.append(rl.gae(r, torch.cat([v[b, :16].cpu(), torch.zeros(1)]), 0.99, 0.95)[0])
+    adv = torch.stack(advs).to(dev)
+    adv = (adv - (adv * k).sum() / k.sum()) / (adv[k > 0].std() + 1e-8)
+
+    def plain():
+        lp = lp64(m, ids)
+        o = lp.detach() if old is None else old
+        r = torch.exp(lp - o)
+        pol = -torch.minimum(r * adv, r.clamp(0.8, 1.2) * adv)
+        return (pol * k).sum() / k.sum() + coef * ((o - lp) * k).sum() / k.sum()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-3, abs=1e-3) and seen[0][0] == pytest.approx(loss)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_dpo_step_of_answers_of_two_lengths(dev):
+    m, ref = model(dev), model(dev, seed=3)
+    t = rl.DPOTrainer(m, ref, beta=0.3)
+    c, cm, _ = batch(dev, S=17)
+    r, rm, _ = batch(dev, S=12, seed=5)
+    got, (loss, acc) = stepped_gradients(t, lambda: t.train_step(c, r, cm, rm))
+
+    def plain():
+        f = lambda q, i, k: (lp64(q, i) * k[:, 1:]).sum(-1)
+        with torch.no_grad():
+            rc, rr = f(ref, c, cm), f(ref, r, rm)
+        x = 0.3 * ((f(m, c, cm) - rc) - (f(m, r, rm) - rr))
+        return -torch.nn.functional.logsigmoid(x).mean()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-4 if dev == "cpu" else 2e-2)
+    again = rl.DPOTrainer(model(dev, seed=9), beta=0.3)               # the reference is a copy: every margin is 0 before the first step
+    assert again.train_step(c, r, cm, rm)[0] == pytest.approx(0.6931472, rel=1e-6)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_distill_step(dev):
+    m, teacher = model(dev), model(dev, seed=11)
+    t = rl.DistillTrainer(m, temperature=2.0)
+    ids, mask, _ = batch(dev)
+    top = t.teacher_top(teacher, ids, k=10)
+    assert top[0].dtype == torch.int32 and top[0].shape == (4, 17, 10)
+    got, loss = stepped_gradients(t, lambda: t.train_step(ids, mask, *top))
+
+    def plain():
+        keep = torch.nn.functional.pad(mask[:, 1:], (0, 1)) > 0
+        lq = torch.log_softmax(top[1] / 2, -1)
+        lp = torch.log_softmax(m(ids).float() / 2, -1).gather(-1, top[0].long())
+        kl = (lq.exp() * (lq - lp)).sum(-1)
+        return 4 * kl[keep].mean()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-4) and t.last_loss() == loss
+
+
+class Squashed(torch.nn.Module):
+    """A model whose last operation keeps what it returned: its logits must not be written over."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner, self.cfg, self.flat = inner, inner.cfg, inner.flatten()
+
+    tok_embeddings = property(lambda self: self.inner.tok_embeddings)
+
+    def flatten(self):
+        return self.flat
+
+    def forward(self, ids):
+        return 5 * torch.tanh(self.inner(ids).float() / 5)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_logits_that_the_backward_pass_reads_stay(dev):
+    m = Squashed(model(dev))
+    t = rl.GRPOTrainer(m, group_size=4)
+    ids, mask, _ = batch(dev)
+    rewards = torch.tensor([1.0, 0.2, -0.5, 0.7])
+    got, _ = stepped_gradients(t, lambda: t.train_step(ids, mask, rewards))
+    adv = t.advantages(rewards).to(dev)[:, None]
+    want, _ = plain_gradients(m, lambda: (-(adv * lp64(m, ids)) * mask[:, 1:]).sum(-1).div(mask[:, 1:].sum(-1)).mean())
+    same(got, want * (1 - 0.01 * 0.04), dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_score_tokens(dev):
+    m = model(dev)
+    ids, mask, _ = batch(dev)
+    targets = rl.next_tokens(ids, mask)
+    lp = m.score_tokens(ids, targets)
+    z = m.hidden_states(ids).view(4, 17, -1).double() @ m.lm_head.double().t()
+    want = torch.log_softmax(z, -1).gather(-1, targets.clamp(min=0)[..., None])[..., 0] * (targets != -100)
+    assert lp.shape == ids.shape and not lp.requires_grad and (lp - want).abs().max() < 1e-4
+    assert (rl.score_tokens(m, ids, targets) - want).abs().max() < (1e-4 if dev == "cpu" else 0.1)      # from logits, which are bfloat16 on the GPU
+    h = ED.EvalHarness(m)
+    a, b = ids[0].tolist()[:6], ids[0].tolist()[6:11]
+    assert h._seq_logp(a, b) == pytest.approx(float(m.score_tokens(ids[:1, :11], rl.next_tokens(ids[:1, :11]))[0, 5:10].mean()), rel=1e-5)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_engine_losses(dev):
+    g = torch.Generator().manual_seed(0)
+    z = torch.randn(4, 6, 30, generator=g).to(dev)
+    y = torch.randint(0, 30, (4, 6), generator=g).to(dev)
+    y[:, 0] = -100
+    ids, top = torch.rand(4, 6, 30, generator=g).argsort(-1)[..., :5].to(dev), torch.randn(4, 6, 5, generator=g).to(dev)
+    ids[0, 0] = -1
+    adv = torch.randn(24, generator=g).to(dev)
+    for f, plain in (
+            (lambda t: ED.policy_grad_loss(t, y, adv), lambda t: -(adv.view(4, 6) * lp_of(t, y) * (y != -100)).sum() / (y != -100).sum()),
+            (lambda t: ED.distill_top_loss(t, ids, top, 1.5), lambda t: top_loss(t, ids, top, 1.5)),
+            (lambda t: ED.preference_loss(t, y, beta=0.5), lambda t: -torch.nn.functional.logsigmoid(
+                0.5 * ((lp_of(t, y) * (y != -100)).sum(1)[:2] - (lp_of(t, y) * (y != -100)).sum(1)[2:])).mean())):
+        loss, d = f(z)
+        t = z.double().requires_grad_(True)
+        want = plain(t)
+        want.backward()
+        assert float(getattr(loss, "loss", loss)) == pytest.approx(float(want.detach()), rel=1e-5)
+        assert d.shape == z.shape and (d - t.grad).abs().max() < 1e-6
+
+
+def lp_of(t, y):
+    return torch.log_softmax(t, -1).gather(-1, y.clamp(min=0)[..., None])[..., 0]
+
+
+def top_loss(t, ids, top, tau):
+    keep = ids[..., 0] >= 0
+    lq = torch.log_softmax(top.double() / tau, -1)
+    lp = torch.log_softmax(t / tau, -1).gather(-1, ids.clamp(min=0))
+    return tau ** 2 * (lq.exp() * (lq - lp)).sum(-1)[keep].mean()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_run_of_them(dev):
+    """One round of post-training as it is put together: old log-probabilities by scoring, several policy steps on one rollout in micro-batches, a
+    preference step, a distillation step - eagerly, and on the GPU with the losses of the policy steps in a captured graph; twice, with the same result from the same weights."""
+    def run(graph):
+        m, teacher = model(dev, seed=2), model(dev, seed=4)
+        m.flatten()
+        ids, mask, g = batch(dev, n=8)
+        targets = rl.next_tokens(ids, mask)
+        adv = torch.randn(8, generator=g).to(dev)
+        old = rl.score_tokens(m, ids, targets)
+        ref = teacher.score_tokens(ids, targets)
+        count = (targets != -100).sum().float().reshape(1)
+        z_in = torch.empty(4, 17, 96, dtype=m.tok_embeddings.dtype, device=dev)
+        t_in, a_in, o_in, r_in = targets[:4].clone(), adv[:4].clone(), old[:4].clone(), ref[:4].clone()
+        call = lambda: L.policy_loss_fwd_bwd(z_in, t_in, a_in, o_in, r_in, clip=(0.2, 0.3), kl_coef=0.05, n_valid=count)
+        replay = None
+        if graph:
+            call()
+            torch.cuda.synchronize()
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                res = call()
+            replay = lambda: (gr.replay(), res)[1]
+        losses = []
+        for step in range(3):
+            for half in (slice(0, 4), slice(4, 8)):
+                logits = m(ids[half])
+                for dst, src in ((z_in, logits.detach()), (t_in, targets[half]), (a_in, adv[half]), (o_in, old[half]), (r_in, ref[half])):
+                    dst.copy_(src)
+                o = replay() if replay else call()
+                logits.backward(o.dlogits.clone())
+                losses.append(o.loss.clone())
+            with torch.no_grad():
+                m.flat.params.sub_((0.05 * m.flat.grads).to(m.flat.params.dtype))
+                m.flat.grads.zero_()
+        d = rl.DPOTrainer(m, teacher)
+        losses.append(torch.tensor(d.train_step(ids[:4], ids[4:], mask[:4], mask[4:])[0]))
+        k = rl.DistillTrainer(m)
+        losses.append(torch.tensor(k.train_step(ids, mask, *k.teacher_top(teacher, ids, 8))))
+        return torch.stack([l.float().cpu() for l in losses]), m.flat.params.clone()
+    first, second = run(False), run(dev == "cuda")
+    assert first[0].isfinite().all() and torch.equal(first[0][:2], second[0][:2])
+    if dev == "cpu":
+        assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
+    else:                       # the embedding's gradient is added up in no fixed order: a weight may round to its neighbour (2^-8)
+        assert ((first[0] - second[0]).abs() <= 2e-2 * first[0].abs() + 2e-2).all()

@@ -15,6 +15,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as TF
 
+from ..ops import losses as L
 from ..trainer import training_utils as TU
 from ..trainer.optimizers import build_optimizer
 from ..trainer.schedulers import schedule_lr
@@ -570,15 +571,22 @@ def normalize_rewards(rewards: torch.Tensor) -> RewardStats:
 def policy_grad_loss(logits, labels, advantages, ignore_index: int = -100):
     """REINFORCE surrogate -(A * log pi(label)) averaged over kept rows; advantages per row.  Returns (loss, dlogits)."""
     lg, lab = _rows(logits, labels)
-    adv = advantages.float().reshape(-1)
-    keep = lab != ignore_index
-    n = max(1, int(keep.sum()))
-    lp = torch.log_softmax(lg, -1)
-    lpt = lp.gather(1, lab.clamp(min=0)[:, None])[:, 0]
-    loss = -(adv * lpt * keep).sum() / n
-    onehot = torch.zeros_like(lp).scatter_(1, lab.clamp(min=0)[:, None], 1.0)
-    d = (adv * keep / n)[:, None] * (lp.exp() - onehot)
-    return float(loss), d.view(logits.shape)
+    o = L.policy_loss_fwd_bwd(lg, lab, advantages.float().reshape(-1), clip=None, ignore_index=ignore_index)
+    return float(o.loss), o.dlogits.view(logits.shape)
+
+
+def distill_top_loss(logits, top_ids, top_logits, temperature: float = 1.0):
+    """Distillation from a teacher's top logits [..., K]: temperature^2 times the mean KL over the rows with entries (ids of -1: none).  Returns
+    (loss, dlogits)."""
+    o = L.distill_loss_fwd_bwd(logits.float().reshape(-1, logits.shape[-1]), top_ids.reshape(-1, top_ids.shape[-1]), top_logits.reshape(-1, top_ids.shape[-1]),
+                               temperature=temperature)
+    return float(o.loss), o.dlogits.view(logits.shape)
+
+
+def preference_loss(logits, labels, ref_logp=None, beta: float = 0.1, label_smoothing: float = 0.0, ignore_index: int = -100):
+    """Loss of N pairs (logits [2N, S, V], labels [2N, S]: chosen answers first).  Returns (LossOut with the share of pairs in the right order, dlogits)."""
+    o = L.preference_loss_fwd_bwd(logits.float(), labels, ref_logp, beta=beta, label_smoothing=label_smoothing, ignore_index=ignore_index)
+    return LossOut(float(o.loss), float((o.margins > 0).float().mean())), o.dlogits
 
 
 @dataclass
@@ -663,10 +671,12 @@ class EvalHarness:
     def _seq_logp(self, ctx: Sequence[int], cont: Sequence[int]) -> float:
         dev = next(self.model.parameters()).device
         ids = torch.tensor([list(ctx) + list(cont)], device=dev)
+        at = slice(len(ctx) - 1, len(ctx) + len(cont) - 1)
+        targets = torch.full_like(ids, -100)
+        targets[0, at] = ids[0, len(ctx):]
+        score = getattr(self.model, "score_tokens", None) or (lambda ids, targets: L.token_logprobs(self.model(ids).float(), targets))
         with torch.no_grad():
-            lp = torch.log_softmax(self.model(ids).float(), -1)[0]
-        pos = torch.arange(len(ctx) - 1, len(ctx) + len(cont) - 1, device=dev)
-        return float(lp[pos, ids[0, len(ctx):]].mean())
+            return float(score(ids, targets)[0, at].mean())
 
     def hellaswag(self, contexts, good, bad):
         """Fraction of items whose true ending has the higher mean token log-probability."""

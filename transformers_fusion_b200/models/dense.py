@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from ..ops import functional as F
+from ..ops.losses import linear_logprobs
 from .config import TransformerConfig
 
 
@@ -451,6 +452,12 @@ class DenseModel(nn.Module):
         f = self.hidden_states(ids)
         logits = _LinearFn.apply(f, self.lm_head)
         return logits.view(B, S, -1)
+
+    @torch.no_grad()
+    def score_tokens(self, ids, targets, ignore_index: int = -100):
+        """Log-probabilities of given tokens, float32 [B, S]: position s scores targets[b, s] after ids[b, :s + 1]; 0 where the target is ``ignore_index``.
+        For passes that want no gradient: the logits are never in memory, and positions that are not scored take no part in the head's product."""
+        return linear_logprobs(self.hidden_states(ids).view(*ids.shape, -1), self.lm_head.data, targets, ignore_index)[0]
 
     @torch.no_grad()
     def head_loss_backward(self, h, lab_f, loss_scale: float = 1.0, ignore_index: int = -100, label_smoothing: float = 0.0,

@@ -25,6 +25,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as TF
 
+from ..ops import losses as L
 from .fused_optim import FlatAdamW
 
 
@@ -33,11 +34,31 @@ def collect_params(model):
     return [p for p in model.parameters() if p.requires_grad]
 
 
+def next_tokens(ids, mask=None):
+    """Target of every position of ids [B, S]: the token that follows; -100 behind the last one and, with ``mask`` [B, S] (1 on the tokens that count), where
+    that token does not count."""
+    out = torch.full_like(ids, -100)
+    out[:, :-1] = ids[:, 1:]
+    if mask is not None:
+        out[:, :-1][mask[:, 1:] == 0] = -100
+    return out
+
+
+def _loss_logits(logits):
+    """Logits of a type that the losses take."""
+    return logits if logits.dtype in (torch.bfloat16, torch.float32) else logits.float()
+
+
+def score_tokens(model, ids, targets):
+    """log p(targets[b, t] | ids[b, :t+1]) -> [B, S], 0 where the target is -100.  No graph.  From the logits as the policy's own are: what differs between
+    two models is then not their rounding.  (``DenseModel.score_tokens`` scores without logits in memory.)"""
+    with torch.no_grad():
+        return L.logprobs_fwd(_loss_logits(model(ids)), targets)[0]
+
+
 def token_logprobs(model, ids):
     """log p(ids[:, t+1] | ids[:, :t+1]) for t = 0..S-2 -> [B, S-1] (graph attached)."""
-    logits = model(ids).float()
-    lp = torch.log_softmax(logits[:, :-1], -1)
-    return lp.gather(-1, ids[:, 1:].unsqueeze(-1)).squeeze(-1)
+    return L.token_logprobs(_loss_logits(model(ids)), next_tokens(ids))[:, :-1]
 
 
 class _RLBase:
@@ -47,8 +68,15 @@ class _RLBase:
         self.opt = FlatAdamW(self.flat, lr=lr, betas=(0.9, 0.999), weight_decay=weight_decay, max_grad_norm=max_grad_norm)
         self.steps = 0
 
-    def _backward_and_step(self, loss, grad_scale=1.0):
-        loss.backward()
+    def _forward(self, ids):
+        """(logits with their graph, the same values without it, where their gradient may go).  The models here end in a linear head, whose backward does
+        not read what it returned: the gradient then takes the logits' place.  Another model's logits are left as they are."""
+        logits = _loss_logits(self.model(ids))
+        z = logits.detach()
+        return logits, z, z if hasattr(self.model, "score_tokens") else None
+
+    def _backward_and_step(self, logits, dlogits, grad_scale=1.0):
+        logits.backward(dlogits)
         for p in self.flat.params_list:      # tensors that went through plain autograd
             if p.grad is not None:
                 p.main_grad.add_(p.grad.float())
@@ -69,8 +97,7 @@ class _RLBase:
     @staticmethod
     def compute_log_probs(logits, ids):
         """log p of the tokens that follow: logits [B, S, V], ids [B, S] -> [B, S-1] (position t scores ids[:, t+1])."""
-        lp = torch.log_softmax(logits.float()[:, :-1], -1)
-        return lp.gather(-1, ids[:, 1:].unsqueeze(-1)).squeeze(-1)
+        return L.token_logprobs(_loss_logits(logits), next_tokens(ids))[:, :-1]
 
     @staticmethod
     def compute_kl_divergence(logits_a, logits_b) -> float:
@@ -137,25 +164,14 @@ class GRPOTrainer(_RLBase):
         self.last_advantages = adv
         if float(rewards.var(unbiased=False)) < 1e-12:
             return 0.0                                    # zero-variance group: no update
-        lp = token_logprobs(self.model, ids)              # [G, S-1]
-        m = mask[:, 1:]
-        denom = m.sum(-1).clamp(min=1)
-        if self.clip_eps > 0:
-            old = lp.detach()
-            ratio = torch.exp(lp - old)
-            a = adv[:, None]
-            per_tok = -torch.minimum(ratio * a, ratio.clamp(1 - self.clip_eps, 1 + self.clip_eps) * a)
-            seq_loss = (per_tok * m).sum(-1) / denom
-        else:
-            ce = -(lp * m).sum(-1) / denom                # CE_i over completion tokens
-            seq_loss = adv * ce
-        loss = seq_loss.mean()
-        if self.ref_model is not None:
-            with torch.no_grad():
-                ref_lp = token_logprobs(self.ref_model, ids)
-            kl = (torch.exp(ref_lp - lp) - (ref_lp - lp) - 1) * m
-            loss = loss + self.kl_coef * (kl.sum(-1) / denom).mean()
-        self._backward_and_step(loss, grad_scale=1.0 - 0.01 * self.beta)
+        targets = next_tokens(ids, mask)
+        ref = score_tokens(self.ref_model, ids, targets) if self.ref_model is not None else None
+        logits, z, out = self._forward(ids)
+        # the group's tokens are the policy's own: with a clip the ratio is 1, without one the objective is advantage * CE
+        o = L.policy_loss_fwd_bwd(z, targets, adv, None, ref, clip=self.clip_eps if self.clip_eps > 0 else None, kl_coef=self.kl_coef if ref is not None else 0.0,
+                                  mean="sequences", out=out)
+        self._backward_and_step(logits, o.dlogits, grad_scale=1.0 - 0.01 * self.beta)
+        loss = o.loss
         self._last_loss = float(loss.detach())
         return self._last_loss
 
@@ -219,8 +235,6 @@ class PPOTrainer(_RLBase):
         dev = self.model.tok_embeddings.device
         ids, mask = ids.to(dev), mask.to(dev).float()
         m = mask[:, 1:]
-        lp = token_logprobs(self.model, ids)
-        old = lp.detach() if old_logprobs is None else old_logprobs.to(dev)
         v = self.values(ids)
         advs, rets = [], []
         for b in range(ids.shape[0]):
@@ -234,25 +248,27 @@ class PPOTrainer(_RLBase):
         adv = torch.stack(advs).to(dev)
         ret = torch.stack(rets).to(dev)
         adv = (adv - (adv * m).sum() / m.sum().clamp(min=1)) / (adv[m > 0].std() + 1e-8 if (m > 0).sum() > 1 else 1.0)
-        ratio = torch.exp(lp - old)
-        pol = -torch.minimum(ratio * adv, ratio.clamp(1 - self.clip, 1 + self.clip) * adv)
-        approx_kl = ((old - lp) * m).sum() / m.sum().clamp(min=1)
-        loss = (pol * m).sum() / m.sum().clamp(min=1) + self.kl_coef * approx_kl
-        self._backward_and_step(loss)
+        targets = next_tokens(ids, mask)
+        pad = lambda t: TF.pad(t.float(), (0, 1))
+        logits, z, out = self._forward(ids)
+        old = L.logprobs_fwd(z, targets)[0] if old_logprobs is None else pad(old_logprobs.to(dev))
+        o = L.policy_loss_fwd_bwd(z, targets, pad(adv), old, old, clip=self.clip, kl_coef=self.kl_coef, kl="k1", out=out)
+        loss, lp = o.loss, o.logp[:, :-1]
+        self._backward_and_step(logits, o.dlogits)
         vloss = (((self.values(ids)[:, :-1] - ret) ** 2) * m).sum() / m.sum().clamp(min=1)
         self.value_opt.zero_grad()
         (self.value_coef * vloss).backward()
         self.value_opt.step()
-        kl = self._last_kl = float(approx_kl.detach())
+        kl = self._last_kl = float(o.kl)
         if getattr(self, "log_cb", None):
             # policy loss, value loss, mean entropy estimate of the action tokens (-log-prob of the taken actions), KL to the old policy
-            ent = float((-(lp.detach()) * m).sum() / m.sum().clamp(min=1))
-            self.log_cb(float(loss.detach()), float(vloss.detach()), ent, kl)
+            ent = float((-lp * m).sum() / m.sum().clamp(min=1))
+            self.log_cb(float(loss), float(vloss.detach()), ent, kl)
         if kl > 1.5 * self.kl_target:                 # adaptive KL coefficient
             self.kl_coef *= 1.5
         elif kl < self.kl_target / 1.5:
             self.kl_coef /= 1.5
-        return float(loss.detach()), float(vloss.detach()), kl
+        return float(loss), float(vloss.detach()), kl
 
 
 # ------------------------------------------------------------------------------------------------
@@ -271,19 +287,55 @@ class DPOTrainer(_RLBase):
     def train_step(self, chosen, rejected, chosen_mask, rejected_mask):
         dev = self.model.tok_embeddings.device
 
-        def seq_lp(model, ids, mask):
-            return (token_logprobs(model, ids.to(dev)) * mask.to(dev).float()[:, 1:]).sum(-1)
-        pc, pr = seq_lp(self.model, chosen, chosen_mask), seq_lp(self.model, rejected, rejected_mask)
-        with torch.no_grad():
-            rc, rr = seq_lp(self.ref, chosen, chosen_mask), seq_lp(self.ref, rejected, rejected_mask)
-        margin = self.beta * ((pc - rc) - (pr - rr))
-        loss = -TF.logsigmoid(margin).mean()
-        self._backward_and_step(loss)
-        self._last_loss = float(loss.detach())
+        # one batch: the chosen answers, then the rejected ones, padded to one length
+        S = max(chosen.shape[1], rejected.shape[1])
+        pad = lambda t: TF.pad(t.to(dev), (0, S - t.shape[1]))
+        ids, mask = torch.cat([pad(chosen), pad(rejected)]), torch.cat([pad(chosen_mask), pad(rejected_mask)])
+        targets = next_tokens(ids, mask)
+        ref = score_tokens(self.ref, ids, targets).sum(-1)
+        logits, z, out = self._forward(ids)
+        o = L.preference_loss_fwd_bwd(z, targets, ref, beta=self.beta, out=out)
+        self._backward_and_step(logits, o.dlogits)
+        self._last_loss = float(o.loss)
+        n = chosen.shape[0]
         if getattr(self, "log_cb", None):
             # loss and the sequence-level KL estimate to the frozen reference on the chosen answers
-            self.log_cb(self._last_loss, float((pc.detach() - rc).mean()))
-        return self._last_loss, float((margin > 0).float().mean())
+            self.log_cb(self._last_loss, float((o.logp[:n] - ref[:n]).mean()))
+        return self._last_loss, float((o.margins > 0).float().mean())
+
+
+# ------------------------------------------------------------------------------------------------
+# distillation
+# ------------------------------------------------------------------------------------------------
+class DistillTrainer(_RLBase):
+    """Distillation of the model from a teacher's best tokens: per position K ids with their logits, stored once (``teacher_top``) or taken from an
+    interface that reports top log-probabilities.  The loss is temperature^2 times the KL divergence from the teacher's renormalised top K."""
+
+    def __init__(self, model, tokenizer=None, temperature=2.0, lr=1e-5, weight_decay=0.0, max_grad_norm=1.0):
+        super().__init__(model, tokenizer, lr=lr, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
+        self.temperature = float(temperature)
+        self._last_loss = 0.0
+
+    def last_loss(self) -> float: return self._last_loss
+
+    @staticmethod
+    def teacher_top(teacher, ids, k: int = 64):
+        """(ids [B, S, k] int32, logits [B, S, k] float32) of the teacher's best tokens behind every position."""
+        with torch.no_grad():
+            top = teacher(ids).float().topk(min(k, L.MAX_TOP), -1)
+        return top.indices.int(), top.values
+
+    def train_step(self, ids, mask, top_ids, top_logits):
+        """ids, mask [B, S] (1 on the tokens that are learnt), top_ids, top_logits [B, S, K]: position s predicts token s + 1.  Returns the loss."""
+        dev = self.model.tok_embeddings.device
+        ids = ids.to(dev)
+        keep = next_tokens(ids, mask.to(dev)) != -100
+        top_ids = torch.where(keep[..., None], top_ids.to(dev), torch.full((), -1, dtype=top_ids.dtype, device=dev))
+        logits, z, out = self._forward(ids)
+        o = L.distill_loss_fwd_bwd(z, top_ids, top_logits.to(dev), temperature=self.temperature, out=out)
+        self._backward_and_step(logits, o.dlogits)
+        self._last_loss = float(o.loss)
+        return self._last_loss
 
 
 # ------------------------------------------------------------------------------------------------
