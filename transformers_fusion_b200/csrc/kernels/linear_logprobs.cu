@@ -42,7 +42,7 @@ struct ScoreArg {
   float* stats;                        // few rows: [2, M]
 };
 
-constexpr int GATHER_ROWS = 32;
+constexpr int GATHER_ROWS = 8;      // a warp to a row
 
 // Which place a row gets depends on the order in which blocks arrive; what is computed for it does not.
 __global__ void __launch_bounds__(256) score_gather_kernel(const ScoreArg a) {
@@ -51,56 +51,54 @@ __global__ void __launch_bounds__(256) score_gather_kernel(const ScoreArg a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * GATHER_ROWS;
   if (warp == 0) {
     const int row = r0 + lane;
-    const bool on = row < a.M && ld_idx(a.targets, row, a.idx64) != a.ignore;
+    const bool mine = lane < GATHER_ROWS && row < a.M, on = mine && ld_idx(a.targets, row, a.idx64) != a.ignore;
     const unsigned mask = __ballot_sync(~0u, on);
     int base = 0;
     if (lane == 0 && mask) base = atomicAdd(a.rows, __popc(mask));
     base = __shfl_sync(~0u, base, 0);
     const int at = base + __popc(mask & ((1u << lane) - 1));
-    place[lane] = on ? at : -1;
+    if (lane < GATHER_ROWS) place[lane] = on ? at : -1;
     if (on) a.row_of[at] = row;
-    else if (row < a.M) a.logp[row] = a.lse[row] = 0.f;
+    else if (mine) a.logp[row] = a.lse[row] = 0.f;
   }
   __syncthreads();
-  for (int i = warp; i < GATHER_ROWS; i += 8) {
-    const int at = place[i];
-    if (at < 0) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(a.x + (r0 + i) * a.ldx);
-    uint4* dst = reinterpret_cast<uint4*>(a.xc + at * a.ldc);
-    for (int v = lane; v < a.H / 8; v += 32) dst[v] = src[v];
-  }
+  const int at = place[warp];
+  if (at < 0) return;
+  const uint4* src = reinterpret_cast<const uint4*>(a.x + (r0 + warp) * a.ldx);
+  uint4* dst = reinterpret_cast<uint4*>(a.xc + at * a.ldc);
+#pragma unroll 8
+  for (int v = lane; v < a.H / 8; v += 32) dst[v] = src[v];
 }
 
-// x[row] . w[target] by a warp; NaN for a target outside the vocabulary
-__device__ __forceinline__ float target_logit(const ScoreArg& a, long long row, int lane) {
+// A thread's share of x[row] . w[target]; NaN for a target outside the vocabulary.
+__device__ __forceinline__ float target_logit(const ScoreArg& a, long long row, int tid, int nt) {
   const long long y = ld_idx(a.targets, row, a.idx64);
   const bool in = y >= 0 && y < a.V;
-  if (lane == 0) TFB_BOUNDS(in, 3, y, a.V);
-  float z = NAN;                     // a target outside the vocabulary
-  if (in) {
-    const uint4 *p = reinterpret_cast<const uint4*>(a.x + row * a.ldx), *q = reinterpret_cast<const uint4*>(a.w + y * a.ldw);
-    float2 t = make_float2(0.f, 0.f), u = t;
-#pragma unroll 4
-    for (int v = lane; v < a.H / 8; v += 32) {
-      const uint4 f = p[v], g = q[v];
-      t = fma2(unpack_bf16(f.x), unpack_bf16(g.x), t);
-      u = fma2(unpack_bf16(f.y), unpack_bf16(g.y), u);
-      t = fma2(unpack_bf16(f.z), unpack_bf16(g.z), t);
-      u = fma2(unpack_bf16(f.w), unpack_bf16(g.w), u);
-    }
-    z = (t.x + u.x) + (t.y + u.y);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(~0u, z, o);
+  if (tid == 0) TFB_BOUNDS(in, 3, y, a.V);
+  if (!in) return NAN;
+  const uint4 *p = reinterpret_cast<const uint4*>(a.x + row * a.ldx), *q = reinterpret_cast<const uint4*>(a.w + y * a.ldw);
+  float2 t = make_float2(0.f, 0.f), u = t;
+#pragma unroll 8
+  for (int v = tid; v < a.H / 8; v += nt) {
+    const uint4 f = p[v], g = q[v];
+    t = fma2(unpack_bf16(f.x), unpack_bf16(g.x), t);
+    u = fma2(unpack_bf16(f.y), unpack_bf16(g.y), u);
+    t = fma2(unpack_bf16(f.z), unpack_bf16(g.z), t);
+    u = fma2(unpack_bf16(f.w), unpack_bf16(g.w), u);
   }
-  return z;
+  return (t.x + u.x) + (t.y + u.y);
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
 }
 
-// R rows to a block, 256 / R threads to a row's parts, eight loads under way in each.  Four rows (of which a part's entries are one 32-byte sector) while
-// there are few: a row of a vocabulary of 128256 has 2004 parts, which take sixteen threads 75 us one by one.
-template <int R>
+// Eight rows to a block (two sectors of a part's entries), 32 threads to a row's parts with eight loads under way in each: a row of a vocabulary of 128256 has 1002 or 2004
+// parts, and one by one they take sixteen threads 75 us.
 __global__ void __launch_bounds__(256) score_finish_kernel(const ScoreArg a) {
   tfb::pdl_sync();
-  constexpr int SHARES = 256 / R, U = 8;
+  constexpr int R = 8, SHARES = 256 / R, U = 8;
   const int n = *a.rows, r0 = blockIdx.x * R;
   if (r0 >= n) return;
   __shared__ float2 sh[SHARES][R];
@@ -126,7 +124,7 @@ __global__ void __launch_bounds__(256) score_finish_kernel(const ScoreArg a) {
   }
   for (int i = warp; i < R && r0 + i < n; i += 8) {
     const int row = a.row_of[r0 + i];
-    const float z = target_logit(a, row, lane);
+    const float z = warp_sum(target_logit(a, row, lane, 32));
     if (lane == 0) zy[i] = z;
   }
   __syncthreads();
@@ -149,15 +147,17 @@ __global__ void __launch_bounds__(256) score_finish_kernel(const ScoreArg a) {
   }
 }
 
-// The same for rows whose statistics are there: a warp to a row.
-__global__ void __launch_bounds__(256) score_rows_kernel(const ScoreArg a) {
+// The same for rows whose statistics are there: a block to a row.
+__global__ void __launch_bounds__(128) score_rows_kernel(const ScoreArg a) {
   tfb::pdl_sync();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.M) return;
+  __shared__ float sh[4];
+  const int row = blockIdx.x;
   const bool on = ld_idx(a.targets, row, a.idx64) != a.ignore;
-  const float z = on ? target_logit(a, row, lane) : 0.f;
-  if (lane) return;
-  const double m = a.stats[row], ls = a.stats[a.M + row], lp = double(z) - m - ls;
+  const float z = on ? warp_sum(target_logit(a, row, threadIdx.x, 128)) : 0.f;
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = z;
+  __syncthreads();
+  if (threadIdx.x) return;
+  const double m = a.stats[row], ls = a.stats[a.M + row], lp = double((sh[0] + sh[1]) + (sh[2] + sh[3])) - m - ls;
   a.lse[row] = float(m + ls);
   a.logp[row] = lp > 0.0 ? 0.f : float(lp);
 }
@@ -183,7 +183,7 @@ TFB_API int tfb_linear_logprobs(const ScoreArg* p, int* status, void* stream) {
     if (rc != TFB_NOT_TAKEN) {
       if (!rc) rc = row_stats(p->z, p->ldz, p->M, p->V, p->targets, p->idx64, p->ignore, p->stats, status, stream);
       if (rc) return rc;
-      tfb::launch_k_rows(p->M, score_rows_kernel, (p->M + 7) / 8, 256, 0, st, *p);
+      tfb::launch_k_pdl(score_rows_kernel, p->M, 128, 0, st, *p);
       return int(cudaGetLastError());
     }
   }
@@ -192,7 +192,6 @@ TFB_API int tfb_linear_logprobs(const ScoreArg* p, int* status, void* stream) {
   ScoreArg a = *p;
   a.parts = gemm_row_stats(p->xc, p->ldc, p->w, p->ldw, p->M, p->V, p->H, p->rows, p->part, status, stream);
   if (a.parts <= 0) return a.parts <= -1000 ? -1000 - a.parts : a.parts;
-  if (p->M <= 2048) tfb::launch_k(score_finish_kernel<4>, (p->M + 3) / 4, 256, 0, st, a);
-  else tfb::launch_k(score_finish_kernel<16>, (p->M + 15) / 16, 256, 0, st, a);
+  tfb::launch_k(score_finish_kernel, (p->M + 7) / 8, 256, 0, st, a);
   return int(cudaGetLastError());
 }

@@ -450,7 +450,8 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
 // ---------------------------------------------------------------------------------------------------------------------
 // The pipelined form: a cluster of C blocks takes a row, each a slice of it that passes through shared memory once, so the row is read once and its
 // gradient written once.  One persistent block per SM, whose warps work on different rows at a time:
-//   producer (1 warp)    bulk copies of 16 KB chunks into a ring, as far ahead as the ring is free
+//   producers (2 warps)  bulk copies of 16 KB chunks into a ring, as far ahead as the ring is free; a chunk to each in turn, since one warp takes ~400 ns for a
+//                        chunk beside twenty busy ones
 //   statistics (2 groups of 4 warps, 4 groups where no gradient follows)   (m, s) of the slice; the groups take chunks in turn, so that one's loads and joins
 //                        run beside another's exponentials
 //   control (4 warps)    rows in turn: joins the warps' and the cluster's (m, s), computes the loss, leaves the two scalars of the gradient
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
 // result depends on the shapes alone (and the GPU).
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int PIPE_W = 4, PIPE_SG = 2, PIPE_GG = 2;                      // warps of a group, groups of statistics, of gradients
-constexpr int PIPE_S = PIPE_SG * PIPE_W, PIPE_G = PIPE_GG * PIPE_W, PIPE_C = 4, PIPE_WARPS = PIPE_S + PIPE_G + PIPE_C + 1, PIPE_CLUSTERS = 148 * 2;
+constexpr int PIPE_S = PIPE_SG * PIPE_W, PIPE_G = PIPE_GG * PIPE_W, PIPE_C = 4, PIPE_P = 2, PIPE_WARPS = PIPE_S + PIPE_G + PIPE_C + PIPE_P, PIPE_CLUSTERS = 148 * 2;
 constexpr int CHUNK_VECS = 1024, CHUNK_BYTES = CHUNK_VECS * 16, PIPE_CHUNKS = 12, PIPE_ROWS = 16, LANE_VECS = 4, HALVES = CHUNK_VECS / (PIPE_W * 32 * LANE_VECS);
 
 struct PipeArg {
@@ -563,7 +564,11 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
   }
   __syncthreads();
   if (C > 1) cluster_sync();           // the others' barriers are set up
-  tfb::pdl_sync();
+  // Behind row_count_kernel, which has waited for everything before it when it lets this kernel start, only its own results have to be waited for: the
+  // denominators (control warps) and the counter (at the end).  Rows are under way meanwhile.  (That kernel itself starts after its predecessor: placed early, its block kept
+  // an SM from the rows; distillation at 12500 x 32000 344 us instead of 322.)
+  constexpr bool COUNTED = MODE == MODE_POLICY || MODE == MODE_DISTILL;
+  if (!COUNTED || (warp >= PIPE_S + PIPE_G && warp < PIPE_WARPS - PIPE_P)) tfb::pdl_sync();
   if (a.zero && blockIdx.x == 0 && threadIdx.x == 0) *a.zero = 0;
 
   auto rows_from = [&](long long base) {
@@ -585,8 +590,8 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
   // waits of a whole warp; `use`: how often the barrier has been waited for before
   auto wait = [&](uint32_t bar, unsigned use, int code) { return mbar_wait_warp(bar, use & 1u, abort_flag, r.status, code); };
 
-  if (warp == PIPE_WARPS - 1) {
-    // ------------------------------ producer ------------------------------
+  if (warp >= PIPE_WARPS - PIPE_P) {
+    // ------------------------------ producers ------------------------------
     unsigned cc = 0;                   // chunks issued
     Cursor c;
     bool ok = true;
@@ -613,6 +618,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
         const T ve_next = edge_value(next, ge_next);
         for (int c0 = 0; c0 < s.n; c0 += CHUNK_VECS, ++cc, c.next(NCH)) {
           const uint32_t slot = c.slot;
+          if (int(slot % PIPE_P) != warp - (PIPE_WARPS - PIPE_P)) continue;
           if (cc >= unsigned(NCH) && !(ok = wait(empty + slot * 8, c.use ^ 1u, ST_TIMEOUT_EMPTY))) break;
           if (__any_sync(~0u, ge >= c0 && ge < c0 + CHUNK_VECS)) {
             if (ge >= c0 && ge < c0 + CHUNK_VECS) reinterpret_cast<T*>(dyn + slot * CHUNK_BYTES)[(ge - c0) * N + xe] = ve;
@@ -637,7 +643,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
       // unwinding: copies in flight land before shared memory goes away
       const uint64_t t0 = globaltimer_ns();
       for (unsigned i = cc > unsigned(NCH) ? cc - NCH : 0; i < cc; ++i)
-        while (!mbar_try_wait(full + (i % NCH) * 8, (i / NCH) & 1u) && globaltimer_ns() - t0 < 2000000ull) {}
+        while (int(i % NCH % PIPE_P) == warp - (PIPE_WARPS - PIPE_P) && !mbar_try_wait(full + (i % NCH) * 8, (i / NCH) & 1u) && globaltimer_ns() - t0 < 2000000ull) {}
     }
   } else if (warp < SW) {
     // ------------------------------ statistics ------------------------------
@@ -927,6 +933,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
   }
   __syncthreads();
   if (q.nsums && rank == 0 && warp == 0) {
+    tfb::pdl_wait();
     int last = 0;
     if (lane == 0) {
       for (int j = 0; j < q.nsums; ++j) {
@@ -967,6 +974,7 @@ __global__ void __launch_bounds__(1024) row_count_kernel(const void* idx, int id
   if (per_seq) {
     for (int n = blockIdx.x * 32 + warp; n < N; n += gridDim.x * 32) {
       int c = 0;
+#pragma unroll 8
       for (int i = lane; i < S; i += 32) c += counts((long long)n * S + i);
       c = __reduce_add_sync(~0u, c);
       if (lane == 0) denom[n] = float(max(c, 1));
@@ -1048,27 +1056,48 @@ __device__ void pair_mean(const PairArg& a, double* sh) {
   if (!last) return;
   __threadfence();
   double v = 0.0;
-  for (int n = threadIdx.x; n < a.N; n += 256) v += double(__ldcg(a.terms + n));
+  for (int n = threadIdx.x; n < a.N; n += 512) v += double(__ldcg(a.terms + n));
   v = block_sum(v, sh);
   if (threadIdx.x == 0) *a.loss = float(v);
 }
 
-__global__ void __launch_bounds__(256) pair_kernel(const PairArg a) {
+__global__ void __launch_bounds__(512) pair_kernel(const PairArg a) {
   tfb::pdl_sync();
   __shared__ double sh[32];
+  __shared__ int count[16];
   const int n = blockIdx.x;
-  double L[2], cnt[2];
-  for (int h = 0; h < 2; ++h) {
-    const long long t0 = (long long)(n + h * a.N) * a.S;
-    double v = 0.0, c = 0.0;
-    for (int i = threadIdx.x; i < a.S; i += 256) {
+  // half of the block to either answer; its sum in 64 bits, in a fixed order
+  const int side = threadIdx.x >> 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  {
+    const long long t0 = (long long)(n + side * a.N) * a.S;
+    double v = 0.0;
+    int c = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x & 255; i < a.S; i += 256) {
       v += a.lp[t0 + i];
-      c += ld_idx(a.targets, t0 + i, a.idx64) != a.ignore ? 1.0 : 0.0;
+      c += ld_idx(a.targets, t0 + i, a.idx64) != a.ignore;
     }
-    L[h] = block_sum(v, sh);
-    cnt[h] = a.average ? fmax(1.0, block_sum(c, sh)) : 1.0;
-    L[h] /= cnt[h];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    c = __reduce_add_sync(~0u, c);
+    if (lane == 0) {
+      sh[warp] = v;
+      count[warp] = c;
+    }
   }
+  __syncthreads();
+  double L[2], cnt[2];
+  if (threadIdx.x == 0)
+    for (int h = 0; h < 2; ++h) {
+      L[h] = 0.0;
+      int c = 0;
+      for (int i = 0; i < 8; ++i) {
+        L[h] += sh[h * 8 + i];
+        c += count[h * 8 + i];
+      }
+      cnt[h] = a.average ? double(max(1, c)) : 1.0;
+      L[h] /= cnt[h];
+    }
   if (threadIdx.x == 0) {
     const double h = (L[0] - (a.ref ? double(a.ref[n]) : 0.0)) - (L[1] - (a.ref ? double(a.ref[a.N + n]) : 0.0));
     const double x = double(a.beta) * h;
@@ -1098,15 +1127,17 @@ __global__ void __launch_bounds__(256) pair_kernel(const PairArg a) {
 
 // The general form's launch.
 template <class T, int MODE>
-static void launch_rows_t(const RowsArg& r, const LossArg& a, bool warp, cudaStream_t st) {
+static void launch_rows_t(const RowsArg& r, const LossArg& a, bool warp, bool pdl, cudaStream_t st) {
   const size_t smem = MODE == MODE_DISTILL ? size_t(a.K) * 8 : 0;
-  if (warp) tfb::launch_k_rows(r.T, row_loss_kernel<T, MODE, true>, (r.T + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, smem * WARP_ROWS, st, r, a);
-  else tfb::launch_k_rows(r.T, row_loss_kernel<T, MODE, false>, r.T, ROW_THREADS, smem, st, r, a);
+  if (warp) tfb::launch_attr(pdl, row_loss_kernel<T, MODE, true>, (r.T + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, smem * WARP_ROWS, st, r, a);
+  else tfb::launch_attr(pdl, row_loss_kernel<T, MODE, false>, r.T, ROW_THREADS, smem, st, r, a);
 }
+// `behind_small`: the kernel before is a small one of this file, so that early-placed blocks take no room from it (see PDL_ROWS otherwise)
 template <int MODE>
-static int launch_rows(const RowsArg& r, const LossArg& a, bool warp, cudaStream_t st) {
-  if (r.f32) launch_rows_t<float, MODE>(r, a, warp, st);
-  else launch_rows_t<__nv_bfloat16, MODE>(r, a, warp, st);
+static int launch_rows(const RowsArg& r, const LossArg& a, bool warp, bool behind_small, cudaStream_t st) {
+  const bool pdl = pdl_mode() == 2 || (pdl_mode() == 1 && (behind_small || r.T <= PDL_ROWS));
+  if (r.f32) launch_rows_t<float, MODE>(r, a, warp, pdl, st);
+  else launch_rows_t<__nv_bfloat16, MODE>(r, a, warp, pdl, st);
   return int(cudaGetLastError());
 }
 
@@ -1167,7 +1198,7 @@ static int launch_pipe_t(const RowsArg& r, const LossArg& a, PipeArg q, long lon
   cudaLaunchAttribute at[2];
   cfg.gridDim = q.clusters * C; cfg.blockDim = PIPE_WARPS * 32; cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = at;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = pdl_mode() == 2 || (pdl_mode() == 1 && r.T <= PDL_ROWS);
+  at[0].val.programmaticStreamSerializationAllowed = pdl_mode() == 2 || (pdl_mode() == 1 && (MODE != MODE_STATS || r.T <= PDL_ROWS));
   cfg.numAttrs = 1;
   if (C > 1) {
     at[1].id = cudaLaunchAttributeClusterDimension;
@@ -1199,11 +1230,11 @@ static int rows_and_sums(const RowsArg& r, LossArg a, int nsums, void* ws, int* 
   int rc = warp ? TFB_NOT_TAKEN : launch_pipe<MODE>(r, a, q, st);
   if (rc != TFB_NOT_TAKEN) return rc;
   a.terms = reinterpret_cast<float*>(static_cast<double*>(ws) + 3 * TERM_BLOCKS);
-  rc = launch_rows<MODE>(r, a, warp, st);
+  rc = launch_rows<MODE>(r, a, warp, MODE != MODE_STATS, st);
   if (rc || !nsums) return rc;
   double* partial = static_cast<double*>(ws);                     // in front of the terms
   const int blocks = min(TERM_BLOCKS, (r.T + 2047) / 2048);
-  tfb::launch_k_rows(r.T, term_sum_kernel, blocks, 512, 0, st, a.terms, r.T, nsums, partial, counter, out);
+  tfb::launch_k_pdl(term_sum_kernel, blocks, 512, 0, st, a.terms, r.T, nsums, partial, counter, out);
   return int(cudaGetLastError());
 }
 
@@ -1238,7 +1269,7 @@ TFB_API int tfb_token_logprobs_bwd(const RowsArg* r, const void* targets, int id
   LossArg a = {};
   a.targets = targets; a.idx64 = idx64; a.ignore = ignore;
   a.stats = const_cast<float*>(stats); a.dlogp = dlogp;
-  return launch_rows<MODE_GRAD>(*r, a, short_rows(*r, a), static_cast<cudaStream_t>(stream));
+  return launch_rows<MODE_GRAD>(*r, a, short_rows(*r, a), false, static_cast<cudaStream_t>(stream));
 }
 
 struct PolicyArg {
@@ -1297,10 +1328,10 @@ TFB_API int tfb_preference_loss(const RowsArg* r, const PreferenceArg* p, void* 
   if (int rc = rows_and_sums<MODE_STATS>(rows, a, 0, nullptr, nullptr, nullptr, st)) return rc;
   PairArg q = {p->lp64, p->targets, p->idx64, p->ignore, p->ref, r->T / r->S / 2, r->S, p->kind, p->average, p->beta, p->smooth, p->logp, p->margins, p->coef, p->terms,
                p->loss, p->counter};
-  tfb::launch_k_rows(r->T, pair_kernel, q.N, 256, 0, st, q);
+  tfb::launch_k_pdl(pair_kernel, q.N, 512, 0, st, q);
   if (!r->dz) return int(cudaGetLastError());
   a.dlogp = p->coef; a.per_seq = 1; a.logp64 = nullptr; a.zero = nullptr;
-  return launch_rows<MODE_GRAD>(*r, a, short_rows(*r, a), st);
+  return launch_rows<MODE_GRAD>(*r, a, short_rows(*r, a), true, st);
 }
 
 struct DistillArg {
