@@ -561,3 +561,104 @@ def test_offsets_past_32_bits():
     check_grad(z[rows], keep, y[rows], -A[rows].double(), BF)
     near(o.logp[rows], torch.log_softmax(keep.double(), -1).gather(1, y[rows, None])[:, 0], 1e-4)
     assert not z[1:700].any() and not z[-5:-1].any()
+
+
+# ------------------------------------------------------------------------------------------------- calls that few make
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [50, 20001])
+def test_reported_kl_and_infinite_margins(dev, V):
+    """A target that the model has masked: its KL estimate is infinite, and has no part in a loss that only reports it; an answer with it is infinitely
+    unlikely, which the sigmoid loss takes without a gradient that is not a number."""
+    z, y = make(dev, (2, 3), V, F32, 1, ignored=0.0)
+    z[0, 1, y[0, 1]] = -math.inf
+    A, ref = torch.ones(2, 3, device=dev), torch.zeros(2, 3, device=dev)
+    old = torch.full((2, 3), -3.0, device=dev)
+    with_ref, without = L.policy_loss_fwd_bwd(z, y, A, old, ref), L.policy_loss_fwd_bwd(z, y, A, old)
+    assert with_ref.kl == math.inf and with_ref.loss.isfinite() and torch.equal(with_ref.loss, without.loss) and torch.equal(with_ref.dlogits, without.dlogits)
+    o = L.preference_loss_fwd_bwd(z, y)                       # the chosen answer is impossible
+    assert o.margins[0] == -math.inf and o.loss == math.inf and o.dlogits.isfinite().all()
+    o = L.preference_loss_fwd_bwd(z.flip(0), y.flip(0))       # the rejected one is
+    assert o.margins[0] == math.inf and o.loss == 0 and not o.dlogits.any()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_inputs_with_a_graph(dev):
+    """Raw calls take no part in autograd: logits that want a gradient may be given, and may be written over."""
+    z, y = make(dev, (2, 4), 40, F32, 2)
+    A = torch.ones(2, 4, device=dev)
+    leaf = z.clone().requires_grad_(True)
+    want = [L.policy_loss_fwd_bwd(z, y, A), L.preference_loss_fwd_bwd(z, y), L.distill_loss_fwd_bwd(z, y[..., None].clamp(min=0), A[..., None])]
+    got = [L.policy_loss_fwd_bwd(leaf, y, A), L.preference_loss_fwd_bwd(leaf, y), L.distill_loss_fwd_bwd(leaf, y[..., None].clamp(min=0), A[..., None])]
+    for a, b in zip(got, want):
+        assert not a.loss.requires_grad and torch.equal(a.loss, b.loss) and torch.equal(a.dlogits, b.dlogits)
+    assert L.policy_loss_fwd_bwd(leaf, y, A, out=leaf).dlogits is leaf and torch.equal(leaf.detach(), want[0].dlogits)
+    hidden = torch.randn(3, 5, 8, device=dev, requires_grad=True)
+    logits = hidden @ torch.randn(8, 40, device=dev)
+    o = L.policy_loss_fwd_bwd(logits, torch.zeros(3, 5, dtype=torch.int64, device=dev), torch.ones(3, 5, device=dev))
+    logits.backward(o.dlogits)
+    assert hidden.grad.isfinite().all() and hidden.grad.any()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,K", [(260, 200), (5001, 3), (40003, 50), (300000, 1000)])
+def test_distill_into_rows_of_another_alignment(dev, dtype, V, K):
+    """Gradient rows that start elsewhere in a vector than the logits'; many entries for short rows; long rows with many entries."""
+    g = gen("cpu", V)
+    z = (2 * torch.randn(3, V, generator=g)).to(dtype).to(dev)
+    ids, top = torch.randint(0, V, (3, K), generator=g).to(dev), torch.randn(3, K, generator=g).to(dev)
+    a = L.distill_loss_fwd_bwd(z, ids, top, temperature=1.5)
+    out = torch.full((3 * (V + 1) + 3,), 9.0, dtype=dtype, device=dev)[3:].view(3, V + 1)[:, :V]
+    b = L.distill_loss_fwd_bwd(z, ids, top, temperature=1.5, out=out)
+    z64 = z.double().requires_grad_(True)
+    q = torch.softmax(top.double() / 1.5, -1)
+    kl = (q * (q.log() - torch.log_softmax(z64 / 1.5, -1).gather(-1, ids))).sum(-1)
+    loss = 1.5 ** 2 * kl.mean()
+    (want,) = torch.autograd.grad(loss, z64)
+    back = torch.zeros_like(want).scatter_add_(-1, ids, q)
+    tol = half(dtype) * want.abs() * (1 + REL) + REL * 0.5 * (torch.softmax(z64.detach() / 1.5, -1) + back) + TINY
+    for o in (a, b):
+        near(o.dlogits, want, tol)
+        near(o.loss, loss.detach(), 2e-5 * (1 + loss.item()))
+    assert bool((out.as_strided((3, 1), (V + 1, 1), out.storage_offset() + V) == 9).all())
+
+
+@pytest.mark.gpu
+def test_scoring_of_many_rows():
+    """More rows than one launch takes, most of them not scored."""
+    M, H, V = L.SCORE_ROWS + 300, 64, 500
+    g = gen("cuda", 3)
+    x, w = torch.randn(M, H, generator=g, device="cuda").to(BF), torch.randn(V, H, generator=g, device="cuda").to(BF)
+    y = torch.randint(0, V, (M,), generator=g, device="cuda")
+    y[torch.rand(M, generator=g, device="cuda") < 0.9] = IGN
+    y[-1], y[0] = 7, IGN
+    lp, lse = L.linear_logprobs(x, w, y)
+    z = x.double() @ w.double().t()
+    keep = y != IGN
+    near(lp, torch.log_softmax(z, -1).gather(1, y.clamp(min=0)[:, None])[:, 0] * keep, 1e-4 * keep)
+    near(lse, torch.logsumexp(z, -1) * keep, 1e-4 * keep)
+    again = L.linear_logprobs(x, w, y)
+    assert torch.equal(again[0], lp) and torch.equal(again[1], lse)
+    for m in (1, 61, 100, 2000):                              # few rows, and the same twice
+        a, b = L.linear_logprobs(x[:m], w, y[:m].clamp(min=0)), L.linear_logprobs(x[:m], w, y[:m].clamp(min=0))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,T", [(32000, 600), (50257, 400), (128256, 300), (3000, 900), (260, 3000)])
+def test_repeats_bit_for_bit(V, T):
+    """Rings, exchanges between blocks and sums in the same order: ten calls beside other work on another stream give the same bits."""
+    z, y = make("cuda", (T,), V, BF, V)
+    A, old = torch.randn(T, device="cuda"), torch.randn(T, device="cuda") - 9
+    ids, top = torch.randint(0, V, (T, 12), device="cuda"), torch.randn(T, 12, device="cuda")
+    side, noise = torch.cuda.Stream(), torch.empty(1 << 26, device="cuda")
+    first = None
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            noise.add_(1)
+        lp, st = L.logprobs_fwd(z, y)
+        p, d = L.policy_loss_fwd_bwd(z, y, A, old, old, kl_coef=0.1), L.distill_loss_fwd_bwd(z, ids, top)
+        got = [lp, st, p.loss, p.kl, p.clipped, p.logp, p.dlogits, d.loss, d.kl, d.dlogits]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    _lib.check_status()

@@ -4,7 +4,7 @@ L2-sized write between timed launches, best and median of ``--iters`` launches; 
 fraction of the copy / GEMM peaks when ``--peaks <json>`` (keys hbm_gbs, bf16_tflops) is given.
 
 Kernels: gemm, gemm_nt_wgrad, gemm_fp8, attention_fwd, attention_bwd, rmsnorm, rmsnorm_bwd, swiglu, rope,
-cross_entropy, adamw, paged_decode, sampling, moe_ffn; those of stack models (``STACK_KERNELS``): diff_attention,
+cross_entropy, token_logprobs, policy_loss, preference_loss, distill_loss, linear_logprobs, adamw, paged_decode, sampling, moe_ffn; those of stack models (``STACK_KERNELS``): diff_attention,
 diff_attention_window, attention_fwd_gqa128 (the plain form of the same layer), diff_decode, delta_prep, delta_scan,
 delta_scan_one, gated_norm, delta_prep_step, delta_step, res_norm, glu_silu, rope_append; those of latent attention and the serving
 mixture with the like kernels of the mixture-of-experts decoder (``LATENT_KERNELS``); those of attention with options and gated linear
@@ -22,7 +22,8 @@ import time
 from .common import add_int
 
 KERNELS = ("gemm", "gemm_wgrad", "gemm_fp8", "attention_fwd", "attention_bwd", "rmsnorm", "rmsnorm_bwd", "swiglu", "rope",
-           "cross_entropy", "adamw", "paged_decode", "sampling", "moe_ffn")
+           "cross_entropy", "token_logprobs", "policy_loss", "preference_loss", "distill_loss", "linear_logprobs", "adamw", "paged_decode", "sampling",
+           "moe_ffn")
 STACK_KERNELS = ("diff_attention", "diff_attention_window", "attention_fwd_gqa128", "diff_decode", "delta_prep", "delta_scan", "delta_scan_one",
                  "gated_norm", "delta_prep_step", "delta_step", "res_norm", "glu_silu", "rope_append")
 LATENT_KERNELS = ("head_attn", "attention_fwd_mha128", "latent_decode", "latent_decode_32", "latent_append", "latent_append_step", "head_linear_q",
@@ -413,6 +414,25 @@ def _build(kernel, n, dev, heads=0, shape=None):
         logits = rnd(T, V)
         labels = torch.randint(0, V, (T,), device=dev)
         return (lambda: F.cross_entropy_fwd_bwd(logits, labels)), 0.0, 2 * T * V * 2
+    if kernel in ("token_logprobs", "policy_loss", "preference_loss", "distill_loss", "linear_logprobs"):
+        from ..ops import losses as L
+        T, V = n * 4, 32000
+        targets = torch.randint(0, V, (T,), device=dev)
+        if kernel == "linear_logprobs":
+            x, w = rnd(T, 1024), rnd(V, 1024, scale=0.03)
+            return (lambda: L.linear_logprobs(x, w, targets)), 2.0 * T * 1024 * V, (T + V) * 1024 * 2
+        logits = rnd(T, V)
+        grad = torch.empty_like(logits)
+        if kernel == "token_logprobs":
+            return (lambda: L.logprobs_fwd(logits, targets)), 0.0, T * V * 2
+        if kernel == "preference_loss":
+            pairs, y = logits.view(-1, T // 4, V), targets.view(-1, T // 4)
+            return (lambda: L.preference_loss_fwd_bwd(pairs, y, out=grad.view_as(pairs))), 0.0, 2 * T * V * 2
+        if kernel == "distill_loss":
+            ids, top = torch.randint(0, V, (T, 64), device=dev), rnd(T, 64)
+            return (lambda: L.distill_loss_fwd_bwd(logits, ids, top, temperature=2.0, out=grad)), 0.0, 2 * T * V * 2
+        adv, old = rnd(T, dtype=torch.float32), rnd(T, dtype=torch.float32) - 10
+        return (lambda: L.policy_loss_fwd_bwd(logits, targets, adv, old, old, kl_coef=0.04, out=grad)), 0.0, 2 * T * V * 2
     if kernel == "adamw":
         N = n * n * 16
         p, gr = torch.randn(N, device=dev), torch.randn(N, device=dev)

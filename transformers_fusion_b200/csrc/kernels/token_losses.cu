@@ -143,11 +143,12 @@ __device__ __forceinline__ void policy_terms(const LossArg& a, float lp, float l
   float dkl = 0.f;
   if (a.ref_lp) {
     const float e = expm1f(ref_lp);
-    kl = a.kl_kind == KL_K3 ? e - ref_lp : ref_lp;
+    kl = a.kl_kind == KL_K3 && ref_lp != INFINITY ? e - ref_lp : ref_lp;
     dkl = a.kl_kind == KL_K3 ? -e : -1.f;
   }
-  l = fmaf(a.kl_coef, kl, -s);
-  g = lp != lp ? lp : fmaf(a.kl_coef, dkl, -ds);       // also where the objective's gradient does not depend on lp
+  // a KL term that is only reported has no part in the loss, not even an infinite one; a NaN has, also where the gradient does not depend on lp
+  l = a.kl_coef != 0.f ? fmaf(a.kl_coef, kl, -s) : -s;
+  g = lp != lp ? lp : a.kl_coef != 0.f ? fmaf(a.kl_coef, dkl, -ds) : -ds;
 }
 
 __device__ __forceinline__ void policy_row(const LossArg& a, double lp, long long t, long long b, float& l, float& kl, float& clipped, float& g) {
@@ -1104,7 +1105,9 @@ __global__ void __launch_bounds__(512) pair_kernel(const PairArg a) {
     double l, dl;                        // of h
     if (a.kind == 0) {
       const double e = exp(-fabs(x)), sneg = x >= 0 ? e / (1.0 + e) : 1.0 / (1.0 + e);      // sigmoid(-x)
-      l = log1p(e) + fmax(-x, 0.0) + double(a.smooth) * x;          // -(1 - s) log sig(x) - s log sig(-x)
+      l = log1p(e) + fmax(-x, 0.0);           // -(1 - s) log sig(x) - s log sig(-x)
+      if (a.smooth != 0.f) l += double(a.smooth) * x;      // (x may be infinite)
+      if (x != x) l = x;
       dl = double(a.beta) * (double(a.smooth) - sneg);
     } else if (a.kind == 1) {
       l = fmax(0.0, 1.0 - x);

@@ -29,7 +29,7 @@ from ._lib import c_i, c_ll, c_p, check
 
 MAX_TOP = 1024          # entries of a teacher's row
 PIPE_CLUSTERS = 296     # most clusters of one launch, each with three sums of 8 bytes in the workspace
-SCORE_ROWS = 1 << 15    # rows of one launch of linear_logprobs: bounds its workspace (a row's hidden state, and 8 bytes per 128 of the vocabulary)
+SCORE_ROWS = 1 << 15    # most rows of one launch of linear_logprobs, whose workspace holds their hidden states and 8 bytes a row per 128 of the vocabulary (up to 512 MB)
 
 _KL = {"k3": 0, "k1": 1}
 _MEAN = {"tokens": 0, "sequences": 1, "sum": 2}
@@ -183,7 +183,7 @@ def _row_gradient(y, c, soft, keep, grad):
     """CPU statement: grad = c (onehot(y) - softmax z) on the kept rows."""
     g = -torch.exp(soft[0] - soft[2][..., None])
     g.scatter_add_(-1, y[..., None], torch.ones_like(g[..., :1]))
-    grad.copy_(torch.where(keep[..., None], g * c[..., None], torch.zeros((), dtype=g.dtype)).to(grad.dtype))
+    grad.detach().copy_(torch.where(keep[..., None], g * c[..., None], torch.zeros((), dtype=g.dtype)).to(grad.dtype))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -195,7 +195,7 @@ def logprobs_fwd(logits, targets, ignore_index: int = -100):
     _check_logits(logits)
     targets = _check_index(targets, logits.shape[:-1], "targets", logits.device)
     if not logits.is_cuda:
-        keep, _, lp, (_, m, ls) = _taken(logits, targets, ignore_index)
+        keep, _, lp, (_, m, ls) = _taken(logits.detach(), targets, ignore_index)
         return lp.float(), torch.where(keep, torch.stack([m, ls]), torch.zeros((), dtype=m.dtype)).float()
     lp, stats = _empty(logits.device, *targets.shape), _empty(logits.device, 2, *targets.shape)
     if targets.numel():
@@ -212,8 +212,8 @@ def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=No
     stats = _check_f32(stats, torch.Size((2, *targets.shape)), "stats", logits.device)
     grad = _gradient(logits, out, True)
     if not logits.is_cuda:
-        keep, y, lp, soft = _taken(logits, targets, ignore_index)
-        c = torch.where(lp.isnan(), lp, dlogp.double())
+        keep, y, lp, soft = _taken(logits.detach(), targets, ignore_index)
+        c = torch.where(lp.isnan(), lp, dlogp.detach().double())
         _row_gradient(y, c, soft, keep, grad)
         return grad
     if targets.numel():
@@ -253,6 +253,37 @@ class PolicyLoss(NamedTuple):
     dlogits: Optional[torch.Tensor]
 
 
+@torch.no_grad()
+def _policy_statement(logits, targets, advantages, old, ref, lo, hi, ratio, kl_coef, kl, mean, n_valid, ignore_index, grad):
+    keep, y, lp, soft = _taken(logits, targets, ignore_index)
+    zero = torch.zeros((), dtype=torch.float64)
+    A = (advantages[:, None] if advantages.dim() < targets.dim() else advantages).double().expand(lp.shape)
+    clipped = torch.zeros_like(lp)
+    if ratio:
+        r = torch.exp(lp - old.double()) if old is not None else torch.exp(lp - lp)
+        s = ds = r * A
+        c = r.clamp(1 - lo, 1 + hi) * A
+        clipped = (c < s).double()
+        s, ds = torch.where(c < s, c, s), torch.where(c < s, zero, ds)
+    else:
+        s, ds = A * lp, A
+    k, dk = torch.zeros_like(lp), torch.zeros_like(lp)
+    if ref is not None:
+        x = ref.double() - lp
+        k, dk = (torch.where(x == math.inf, x, torch.expm1(x) - x), -torch.expm1(x)) if kl == "k3" else (x, -torch.ones_like(x))
+    w = keep.double()
+    if mean == "tokens":
+        w = w / (n_valid.double() if n_valid is not None else w.sum().clamp(min=1))
+    elif mean == "sequences":
+        w = w.view(-1, targets.shape[-1])
+        w = (w / (max(len(w), 1) * w.sum(1, keepdim=True).clamp(min=1))).view(keep.shape)
+    total = lambda v: torch.where(keep, w * v, zero).sum().float()
+    loss, dloss = (kl_coef * k - s, kl_coef * dk - ds) if kl_coef != 0 else (-s, -ds)
+    if grad is not None:
+        _row_gradient(y, torch.where(lp.isnan(), lp, w * dloss), soft, keep, grad)
+    return PolicyLoss(total(loss), total(k), total(clipped), lp.float(), grad)
+
+
 def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logprobs=None, *, clip=0.2, kl_coef: float = 0.0, kl: str = "k3",
                         mean: str = "tokens", n_valid=None, ignore_index: int = -100, want_grad: bool = True, out=None) -> PolicyLoss:
     """Policy loss of sampled tokens and its gradient with respect to the logits, in one pass over them.
@@ -262,7 +293,7 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     of lp; without a clip as well the objective is A lp itself.  KL against ``ref_logprobs``, x = ref - lp: "k3" exp(x) - 1 - x (estimates KL(policy || reference)
     on the policy's tokens), "k1" x (KL(reference || policy) on the reference's).
 
-    ``advantages``: one per token, or [B], one per sequence.  ``mean``: over all "tokens" (``n_valid``, one float32 value on the device, replaces their
+    ``advantages``: one per token, or [B], one per sequence.  ``mean``: over all "tokens" (``n_valid``, one float32 value above 0 on the device, replaces their
     number, for a batch in several calls), over the "sequences" of each one's mean over its tokens (a sequence without tokens counts as 0), or "sum"."""
     _check_logits(logits)
     dev = logits.device
@@ -283,32 +314,7 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     grad = _gradient(logits, out, want_grad)
     B, S = targets.shape if targets.dim() == 2 else (1, targets.shape[0])
     if not logits.is_cuda:
-        keep, y, lp, soft = _taken(logits, targets, ignore_index)
-        zero = torch.zeros((), dtype=torch.float64)
-        A = (advantages[:, None] if adv_seq else advantages).double().expand(lp.shape)
-        clipped = torch.zeros_like(lp)
-        if ratio:
-            r = torch.exp(lp - old.double()) if old is not None else torch.exp(lp - lp)
-            s = ds = r * A
-            c = r.clamp(1 - lo, 1 + hi) * A
-            clipped = (c < s).double()
-            s, ds = torch.where(c < s, c, s), torch.where(c < s, zero, ds)
-        else:
-            s, ds = A * lp, A
-        k, dk = torch.zeros_like(lp), torch.zeros_like(lp)
-        if ref is not None:
-            x = ref.double() - lp
-            k, dk = (torch.expm1(x) - x, -torch.expm1(x)) if kl == "k3" else (x, -torch.ones_like(x))
-        w = keep.double()
-        if mean == "tokens":
-            w = w / (n_valid.double() if n_valid is not None else w.sum().clamp(min=1))
-        elif mean == "sequences":
-            w = w.view(B, S)
-            w = (w / (max(B, 1) * w.sum(1, keepdim=True).clamp(min=1))).view(keep.shape)
-        total = lambda v: torch.where(keep, w * v, zero).sum().float()
-        if grad is not None:
-            _row_gradient(y, torch.where(lp.isnan(), lp, w * (kl_coef * dk - ds)), soft, keep, grad)
-        return PolicyLoss(total(kl_coef * k - s), total(k), total(clipped), lp.float(), grad)
+        return _policy_statement(logits, targets, advantages, old, ref, lo, hi, ratio, kl_coef, kl, mean, n_valid, ignore_index, grad)
     lp = _empty(dev, *targets.shape)
     if not lp.numel():
         z = torch.zeros((), device=dev)
@@ -333,6 +339,28 @@ class PreferenceLoss(NamedTuple):
     dlogits: Optional[torch.Tensor]
 
 
+@torch.no_grad()
+def _preference_statement(logits, targets, ref, beta, kind, label_smoothing, average, ignore_index, grad):
+    N = len(targets) // 2
+    keep, y, lp, soft = _taken(logits, targets, ignore_index)
+    n = keep.sum(1).clamp(min=1).double() if average else torch.ones(2 * N, dtype=torch.float64)
+    L = lp.sum(1) / n
+    d = L - (ref.double() if ref is not None else 0)
+    h = d[:N] - d[N:]
+    x = beta * h
+    if kind == "sigmoid":
+        l = torch.log1p(torch.exp(-x.abs())) + (-x).clamp(min=0) + (label_smoothing * x if label_smoothing else 0)
+        dl = beta * (label_smoothing - torch.sigmoid(-x))
+    elif kind == "hinge":
+        l, dl = (1 - x).clamp(min=0), torch.where(x.isnan(), x, -beta * (x < 1).double())
+    else:
+        l, dl = (h - 0.5 / beta) ** 2, 2 * (h - 0.5 / beta)
+    if grad is not None:
+        c = torch.cat([dl, -dl]) / max(N, 1) / n
+        _row_gradient(y, c[:, None].expand(lp.shape), soft, keep, grad)
+    return PreferenceLoss((l.sum() / max(N, 1)).float(), x.float(), L.float(), grad)
+
+
 def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float = 0.1, kind: str = "sigmoid", label_smoothing: float = 0.0,
                             average: bool = False, ignore_index: int = -100, want_grad: bool = True, out=None) -> PreferenceLoss:
     """Loss of N pairs of answers and its gradient: logits [2N, S, V] and targets [2N, S] hold the N chosen answers first, then the N rejected
@@ -355,23 +383,7 @@ def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float =
     ref = _check_f32(ref_logprobs, torch.Size((2 * N,)), "ref_logprobs", dev)
     grad = _gradient(logits, out, want_grad)
     if not logits.is_cuda:
-        keep, y, lp, soft = _taken(logits, targets, ignore_index)
-        n = keep.sum(1).clamp(min=1).double() if average else torch.ones(2 * N, dtype=torch.float64)
-        L = lp.sum(1) / n
-        d = L - (ref.double() if ref is not None else 0)
-        h = d[:N] - d[N:]
-        x = beta * h
-        if kind == "sigmoid":
-            l = torch.log1p(torch.exp(-x.abs())) + (-x).clamp(min=0) + label_smoothing * x
-            dl = beta * (label_smoothing - torch.sigmoid(-x))
-        elif kind == "hinge":
-            l, dl = (1 - x).clamp(min=0), torch.where(x.isnan(), x, -beta * (x < 1).double())
-        else:
-            l, dl = (h - 0.5 / beta) ** 2, 2 * (h - 0.5 / beta)
-        if grad is not None:
-            c = torch.cat([dl, -dl]) / max(N, 1) / n
-            _row_gradient(y, c[:, None].expand(lp.shape), soft, keep, grad)
-        return PreferenceLoss((l.sum() / max(N, 1)).float(), x.float(), L.float(), grad)
+        return _preference_statement(logits, targets, ref, beta, kind, label_smoothing, average, ignore_index, grad)
     margins, L = _empty(dev, N), _empty(dev, 2 * N)
     if N == 0 or S == 0:
         # no pairs, or only empty answers: nothing depends on the logits
@@ -398,6 +410,28 @@ class DistillLoss(NamedTuple):
     dlogits: Optional[torch.Tensor]
 
 
+@torch.no_grad()
+def _distill_statement(logits, top_ids, top_logits, temperature, n_valid, grad):
+    V = logits.shape[-1]
+    ids = top_ids.long()
+    keep, have = ids[..., 0] >= 0, (ids >= 0) & (ids < V)
+    bad = (ids >= V).any(-1) & keep
+    zero = torch.zeros((), dtype=torch.float64)
+    lq = torch.log_softmax(torch.where(have, top_logits.double() / temperature, torch.full((), -math.inf, dtype=torch.float64)), -1)
+    q = torch.where(have, lq.exp(), zero)
+    z, _, ls = _softmax64(logits.double() / temperature)
+    lp = z.gather(-1, ids.clamp(0, V - 1)) - ls[..., None]
+    kl = torch.where(have & (q != 0), q * (lq - lp), zero).sum(-1)
+    kl = torch.where(keep, torch.where(bad, torch.full_like(kl, math.nan), kl), zero)
+    w = 1.0 / (n_valid.double() if n_valid is not None else keep.sum().clamp(min=1).double())
+    if grad is not None:
+        d = torch.exp(z - ls[..., None])
+        d.scatter_add_(-1, ids.clamp(0, V - 1), -q)
+        d = torch.where(bad[..., None], torch.full_like(d, math.nan), d) * (temperature * w)
+        grad.copy_(torch.where(keep[..., None], d, zero).to(grad.dtype))
+    return DistillLoss((kl.sum() * temperature ** 2 * w).float().reshape(()), kl.float(), grad)
+
+
 def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.0, n_valid=None, want_grad: bool = True, out=None) -> DistillLoss:
     """Distillation from the top logits of a teacher, and its gradient, in one pass over the student's logits.
 
@@ -405,7 +439,7 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     tokens of every row with their logits (or log-probabilities: only differences count).  Negative ids are entries that are not there; a row
     whose first id is negative has none and is not trained on.  With q the soft-max of a row's entries at the temperature and p that of the
     student's whole row, KL = sum q (log q - log p); loss = temperature^2 mean KL.  An id that comes twice counts twice.  A row with entries whose
-    teacher logits are all -inf, or with an id outside the vocabulary, gives NaN.  ``n_valid`` (one float32 value on the device) replaces
+    teacher logits are all -inf, or with an id outside the vocabulary, gives NaN.  ``n_valid`` (one float32 value above 0 on the device) replaces
     the number of rows with entries."""
     _check_logits(logits)
     dev, V = logits.device, logits.shape[-1]
@@ -422,23 +456,7 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     grad = _gradient(logits, out, want_grad)
     rows = logits.shape[:-1]
     if not logits.is_cuda:
-        ids = top_ids.long()
-        keep, have = ids[..., 0] >= 0, (ids >= 0) & (ids < V)
-        bad = (ids >= V).any(-1) & keep
-        zero = torch.zeros((), dtype=torch.float64)
-        lq = torch.log_softmax(torch.where(have, top_logits.double() / temperature, torch.full((), -math.inf, dtype=torch.float64)), -1)
-        q = torch.where(have, lq.exp(), zero)
-        z, _, ls = _softmax64(logits.double() / temperature)
-        lp = z.gather(-1, ids.clamp(0, V - 1)) - ls[..., None]
-        kl = torch.where(have & (q != 0), q * (lq - lp), zero).sum(-1)
-        kl = torch.where(keep, torch.where(bad, torch.full_like(kl, math.nan), kl), zero)
-        w = 1.0 / (n_valid.double() if n_valid is not None else keep.sum().clamp(min=1).double())
-        if grad is not None:
-            d = torch.exp(z - ls[..., None])
-            d.scatter_add_(-1, ids.clamp(0, V - 1), -q)
-            d = torch.where(bad[..., None], torch.full_like(d, math.nan), d) * (temperature * w)
-            grad.copy_(torch.where(keep[..., None], d, zero).to(grad.dtype))
-        return DistillLoss((kl.sum() * temperature ** 2 * w).float().reshape(()), kl.float(), grad)
+        return _distill_statement(logits, top_ids, top_logits, temperature, n_valid, grad)
     kl = _empty(dev, *rows)
     T = kl.numel()
     if not T:
@@ -489,7 +507,7 @@ def linear_logprobs(x, weight, targets, ignore_index: int = -100):
     (V, H), M = w.shape, y.numel()
     if not M:
         return lp, lse
-    n = min(M, SCORE_ROWS)
+    n = min(M, SCORE_ROWS, max(256, (1 << 27) // (4 * -(-V // 256))))
     # workspace: parts of a row's statistics (two values per half a tile), compacted rows and their number; the logits of few rows
     ldz = -(-V // 4) * 4 if n <= 128 and n * V <= 1 << 27 else 0
     parts = 4 * -(-V // (128 if n <= 128 else 256)) * n

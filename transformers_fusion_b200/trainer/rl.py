@@ -322,7 +322,8 @@ class DistillTrainer(_RLBase):
     def teacher_top(teacher, ids, k: int = 64):
         """(ids [B, S, k] int32, logits [B, S, k] float32) of the teacher's best tokens behind every position."""
         with torch.no_grad():
-            top = teacher(ids).float().topk(min(k, L.MAX_TOP), -1)
+            logits = teacher(ids).float()
+            top = logits.topk(min(k, L.MAX_TOP, logits.shape[-1]), -1)
         return top.indices.int(), top.values
 
     def train_step(self, ids, mask, top_ids, top_logits):
