@@ -47,7 +47,7 @@ struct LossArg {
   double* logp64;                      // [T], preference
   // MODE_GRAD: coefficient of a row
   const float* dlogp;                  // [T], or [T / S] with per_seq
-  int per_seq;
+  int per_seq, split;                  // blocks of a row
   // MODE_POLICY
   const float *adv, *old_lp, *ref_lp;
   int adv_seq, ratio, kl_kind;
@@ -314,13 +314,14 @@ template <class T, int MODE, bool WARP>
 __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 : MODE == MODE_GRAD ? 4 : 3) row_loss_kernel(const RowsArg r, const LossArg a) {
   tfb::pdl_sync();
   __shared__ float2 sh[32];
-  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : int(blockDim.x), warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5, split = !WARP && MODE == MODE_GRAD ? a.split : 1;
+  const int nt = WARP ? 32 : ROW_THREADS * split, tid = WARP ? threadIdx.x & 31 : threadIdx.x + (split > 1 ? blockIdx.x % split * ROW_THREADS : 0);
   auto sync = [&] { if constexpr (WARP) __syncwarp(); else __syncthreads(); };
   auto join_all = [&](float& m, float& s, float k) { if constexpr (WARP) warp_join(m, s, k); else block_join(m, s, k, sh); };
   extern __shared__ __align__(128) char dyn[];         // MODE_DISTILL: K teacher weights, K ids
   if (a.zero && blockIdx.x == 0 && threadIdx.x == 0) *a.zero = 0;
   // the gradient of given statistics goes from the last row to the first: the pass that took them has left the last ones in L2
-  const long long place = MODE == MODE_GRAD ? gridDim.x - 1 - blockIdx.x : blockIdx.x, t = WARP ? place * WARP_ROWS + warp : place;
+  const long long place = MODE == MODE_GRAD ? (gridDim.x - 1 - blockIdx.x) / split : blockIdx.x, t = WARP ? place * WARP_ROWS + warp : place;
   if (WARP && t >= r.T) return;
   const long long b = t / r.S, pos = t - b * r.S;
   const T* row = static_cast<const T*>(r.z) + b * r.zb + pos * r.zs;
@@ -415,13 +416,13 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
       return;
     }
     if (tid == 0) TFB_BOUNDS(y >= 0 && y < r.V, 3, y, r.V);
-    const float zy = y >= 0 && y < r.V ? Vec<T>::get(row[y]) : NAN;       // a target outside the vocabulary makes its row NaN
+    const bool in = y >= 0 && y < r.V;       // a target outside the vocabulary makes its row NaN
     if constexpr (MODE == MODE_GRAD) {
       const float m = a.stats[t], mr = m == -INFINITY ? 0.f : m, p = ex2(-a.stats[r.T + t] * k);       // 1 / S
-      const float c = zy != zy ? NAN : (a.per_seq ? a.dlogp[b] : a.dlogp[t]);
-      sync();
+      const float c = !in ? NAN : (a.per_seq ? a.dlogp[b] : a.dlogp[t]);
       row_grad(row, out, r.V, k, mr, -c * p, y, -c, tid, nt);
     } else {
+      const float zy = in ? Vec<T>::get(row[y]) : NAN;
       float m, s;
       row_stats<T, 2>(row, r.V, k, m, s, tid, nt);
       join_all(m, s, k);
@@ -1132,8 +1133,15 @@ __global__ void __launch_bounds__(512) pair_kernel(const PairArg a) {
 template <class T, int MODE>
 static void launch_rows_t(const RowsArg& r, const LossArg& a, bool warp, bool pdl, cudaStream_t st) {
   const size_t smem = MODE == MODE_DISTILL ? size_t(a.K) * 8 : 0;
-  if (warp) tfb::launch_attr(pdl, row_loss_kernel<T, MODE, true>, (r.T + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, smem * WARP_ROWS, st, r, a);
-  else tfb::launch_attr(pdl, row_loss_kernel<T, MODE, false>, r.T, ROW_THREADS, smem, st, r, a);
+  if (warp) return tfb::launch_attr(pdl, row_loss_kernel<T, MODE, true>, (r.T + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, smem * WARP_ROWS, st, r, a);
+  LossArg q = a;
+  if (MODE == MODE_GRAD) {
+    // Few rows: several blocks to one, up to two waves of the four that an SM holds, two vectors to a thread at least.  us, so / a block to a row: 10 x 128256
+    // 3.6 / 13.7, 61 x 128256 8.9 / 14.4, 200 x 32000 7.3 / 6.9; with more waves the blocks' starts show (1280 x 32000 37 / 35, 1400 x 50257 59 / 56).
+    const int blocks = 2 * 4 * sm_count(), most = r.V / (Vec<T>::N * ROW_THREADS * 2);
+    q.split = max(1, min((blocks + r.T - 1) / r.T, most));
+  }
+  tfb::launch_attr(pdl, row_loss_kernel<T, MODE, false>, r.T * max(1, q.split), ROW_THREADS, smem, st, r, q);
 }
 // `behind_small`: the kernel before is a small one of this file, so that early-placed blocks take no room from it (see PDL_ROWS otherwise)
 template <int MODE>
