@@ -1422,7 +1422,9 @@ TFB_API int tfb_gemm_glu(const void* A, long long lda, const void* B, long long 
 
 // Statistics of the rows of A . B^T without the product in memory (see GemmParams::part): A [M, K] of which the first *rows rows count, B [N, K].  Returns the
 // number of parts of a row (`part` holds that many x M entries, at most 2 ceil(N / 128)), or an error.
-// Up to one tile of rows B is streamed once, in tiles of 128 columns on single CTAs: SMEMNOTE
+// Up to one tile of rows (128) one half of a pair would have nothing to compute: single CTAs, with tiles of 128 columns.  us, the whole of linear_logprobs: 128 x 32000 x
+// 512 21, 128 x 128256 x 512 45.  More rows take pairs of SMs with tiles of 256 x 256; the product alone takes 2.94 ms for
+// 4390 x 128256 x 4096 (1570 TFLOP/s) and 162 us for 6470 x 32000 x 512 (1310: at that depth the epilogue's exponentials, one to 512 multiply-adds, show).
 int tfb::gemm_row_stats(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const int* rows, float2* part, int* status,
                         void* stream) {
   CUtensorMap ta, tb;
@@ -1436,7 +1438,7 @@ int tfb::gemm_row_stats(const void* A, long long lda, const void* B, long long l
   p.splits = 1;
   p.kb_per_split = (K + BK - 1) / BK;
   p.wg_n_shift = -1;
-  const bool one = M <= BM || sm_count() < 2;
+  const bool one = M <= BM;
   if (int rc = make_tmap_2d(&ta, A, 2, K, M, lda * 2, BK, BM)) return rc;
   const int rows_of_tile = one ? BM : 2 * BM, cols_of_tile = one ? BM : 2 * BM;
   p.tiles_m = (M + rows_of_tile - 1) / rows_of_tile;

@@ -7,8 +7,8 @@
 * ``distill_loss_fwd_bwd``: KL divergence from a teacher's stored top logits.
 * ``linear_logprobs``: log-probabilities of given tokens from hidden states and the head's weight, for passes that want no gradient.
 
-As in ``ops/functional.py``: CUDA tensors go to the sm_100a kernels (``csrc/kernels/token_losses.cu``), CPU tensors run the plain PyTorch
-statement of the same mathematics.
+As in ``ops/functional.py``: CUDA tensors go to the sm_100a kernels (``csrc/kernels/token_losses.cu``, ``linear_logprobs.cu``), CPU
+tensors run the plain PyTorch statement of the same mathematics.
 
 Logits are [T, V] or [B, S, V], bfloat16 or float32, of any strides with a dense last dimension (rows may start at any element).  Targets are
 int64 or int32 of the logits' leading shape; rows whose target is ``ignore_index`` are not read, their statistics and gradients are 0.  A
@@ -29,7 +29,7 @@ from ._lib import c_i, c_ll, c_p, check
 
 MAX_TOP = 1024          # entries of a teacher's row
 PIPE_CLUSTERS = 296     # most clusters of one launch, each with three sums of 8 bytes in the workspace
-SCORE_ROWS = 1 << 15    # most rows of one launch of linear_logprobs, whose workspace holds their hidden states and 8 bytes a row per 128 of the vocabulary (up to 512 MB)
+SCORE_ROWS = 1 << 15    # most rows of one launch of linear_logprobs, whose workspace holds their hidden states and 8 bytes a row per 128 of the vocabulary (512 MB of these)
 
 _KL = {"k3": 0, "k1": 1}
 _MEAN = {"tokens": 0, "sequences": 1, "sum": 2}
@@ -473,9 +473,6 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
 # ---------------------------------------------------------------------------------------------
 # scoring from hidden states
 # ---------------------------------------------------------------------------------------------
-SCORE_ROWS = 1 << 15          # rows of one launch: bounds its workspace (a row's hidden state, and 8 bytes per 128 of the vocabulary)
-
-
 def _tma_ready(t):
     """Rows that start at 16-byte boundaries."""
     if t.stride(-1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
