@@ -307,6 +307,24 @@ __device__ __forceinline__ void row_grad(const T* row, T* out, int V, float k, f
   if (tail + tid < V) one(tail + tid);
 }
 
+// An id may come twice among a teacher's entries, and the gradient at either has the weights of both.  A table of the ids (twice as many places as entries, -1 where
+// empty) tells whether one does, since looking through all of a row's entries for each of them takes K^2 steps.
+__host__ __device__ constexpr int top_table(int K) {
+  int n = 64;
+  while (n < 2 * K) n *= 2;
+  return n;
+}
+__device__ __forceinline__ bool seen_before(int* table, int places, int id) {
+  for (unsigned at = unsigned(id) * 2654435769u >> 16;; ++at) {      // (Knuth's multiplicative hash)
+    const int o = atomicCAS(table + (at & unsigned(places - 1)), -1, id);
+    if (o == -1 || o == id) return o == id;
+  }
+}
+
+// In the general form a warp looks through up to 64 entries as fast: us, so / with the table, 8192 x 2000 20 entries 38 / 46, 64 45 / 53, 128 67 / 67; 20000 x 260 20 entries
+// 44 / 47, 64 58 / 55, 128 113 / 61.
+__host__ __device__ constexpr int row_table(bool warp, int K) { return warp && K <= 64 ? 0 : top_table(K); }
+
 constexpr int ROW_THREADS = 512, WARP_ROWS = 8, WARP_TOP = 128;      // rows of a block, and most entries of a teacher's, with a warp to a row
 
 // WARP: a warp to a row, WARP_ROWS rows to a block; else a block to a row.
@@ -318,7 +336,7 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
   const int nt = WARP ? 32 : ROW_THREADS * split, tid = WARP ? threadIdx.x & 31 : threadIdx.x + (split > 1 ? blockIdx.x % split * ROW_THREADS : 0);
   auto sync = [&] { if constexpr (WARP) __syncwarp(); else __syncthreads(); };
   auto join_all = [&](float& m, float& s, float k) { if constexpr (WARP) warp_join(m, s, k); else block_join(m, s, k, sh); };
-  extern __shared__ __align__(128) char dyn[];         // MODE_DISTILL: K teacher weights, K ids
+  extern __shared__ __align__(128) char dyn[];         // MODE_DISTILL: K teacher weights, K ids, the ids' table
   if (a.zero && blockIdx.x == 0 && threadIdx.x == 0) *a.zero = 0;
   // the gradient of given statistics goes from the last row to the first: the pass that took them has left the last ones in L2
   const long long place = MODE == MODE_GRAD ? (gridDim.x - 1 - blockIdx.x) / split : blockIdx.x, t = WARP ? place * WARP_ROWS + warp : place;
@@ -335,8 +353,10 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
       if (out) row_zero(out, r.V, tid, nt);
       return;
     }
-    float* q = reinterpret_cast<float*>(dyn) + (WARP ? warp * 2 * a.K : 0);
-    int* id = reinterpret_cast<int*>(q + a.K);
+    const int places = row_table(WARP, a.K);
+    float* q = reinterpret_cast<float*>(dyn) + (WARP ? warp * (2 * a.K + places) : 0);
+    int *id = reinterpret_cast<int*>(q + a.K), *table = id + a.K;
+    for (int i = tid; i < places; i += nt) table[i] = -1;
     float m, s;
     row_stats<T, 2>(row, r.V, k, m, s, tid, nt);
     join_all(m, s, k);
@@ -355,16 +375,17 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
     join_all(tm, ts, k);
     const float tr = tm == -INFINITY ? 0.f : tm;
     float kl = 0.f;
-    bool bad = false;
+    bool bad = false, twice = places == 0;
     const float mr = m == -INFINITY ? 0.f : m, ls = logf(s), lts = logf(ts);
     for (int j = tid; j < a.K; j += nt) {
       if (id[j] == -2) bad = true;
       const float lq = (q[j] - tr) * a.inv_tau - lts, w = ex2((q[j] - tr) * k) / ts;
       q[j] = id[j] >= 0 ? w : 0.f;
+      if (places && out && id[j] >= 0) twice |= seen_before(table, places, id[j]);
       if (id[j] >= 0 && q[j] != 0.f) kl += q[j] * (lq - ((Vec<T>::get(row[id[j]]) - mr) * a.inv_tau - ls));
     }
     int any_bad;
-    if constexpr (WARP) { any_bad = __any_sync(~0u, bad); __syncwarp(); } else any_bad = __syncthreads_or(bad);
+    if constexpr (WARP) { any_bad = __any_sync(~0u, bad); twice = __any_sync(~0u, twice); __syncwarp(); } else { any_bad = __syncthreads_or(bad); twice = __syncthreads_or(twice); }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) kl += __shfl_xor_sync(~0u, kl, o);
     if constexpr (!WARP) {
@@ -391,8 +412,8 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
       const int j = tid + u * nt;
       g[u] = 0.f;
       if (j < a.K && id[j] >= 0) {
-        float sum = 0.f;
-        for (int i = 0; i < a.K; ++i) sum += id[i] == id[j] ? q[i] : 0.f;       // an id may come twice
+        float sum = twice ? 0.f : q[j];
+        for (int i = 0; twice && i < a.K; ++i) sum += id[i] == id[j] ? q[i] : 0.f;
         g[u] = c * (ex2((Vec<T>::get(row[id[j]]) - mr) * k) / s - sum);
       }
     }
@@ -476,7 +497,7 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int PIPE_W = 4, PIPE_SG = 2, PIPE_GG = 2;                      // warps of a group, groups of statistics, of gradients
 constexpr int PIPE_S = PIPE_SG * PIPE_W, PIPE_G = PIPE_GG * PIPE_W, PIPE_C = 4, PIPE_P = 2, PIPE_WARPS = PIPE_S + PIPE_G + PIPE_C + PIPE_P, PIPE_CLUSTERS = 148 * 2;
-constexpr int CHUNK_VECS = 1024, CHUNK_BYTES = CHUNK_VECS * 16, PIPE_CHUNKS = 12, PIPE_ROWS = 16, LANE_VECS = 4, HALVES = CHUNK_VECS / (PIPE_W * 32 * LANE_VECS);
+constexpr int CHUNK_VECS = 1024, CHUNK_BYTES = CHUNK_VECS * 16, PIPE_CHUNKS = 12, PIPE_ROWS = 16, TOP_LOADS = 2, LANE_VECS = 4, HALVES = CHUNK_VECS / (PIPE_W * 32 * LANE_VECS);
 
 struct PipeArg {
   int vs, chunks, clusters, csize, nsums;
@@ -532,22 +553,23 @@ static_assert(PIPE_ROWS > PIPE_CHUNKS && PIPE_ROWS >= 2 * PIPE_C && PIPE_ROWS % 
 template <class T, int MODE, bool GRAD>
 __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const RowsArg r, const LossArg a, const PipeArg q) {
   constexpr int N = Vec<T>::N, ES = int(sizeof(T)), LV = LANE_VECS, SGS = GRAD ? PIPE_SG : PIPE_SG + PIPE_GG, SW = SGS * PIPE_W;      // groups and warps of the statistics
-  extern __shared__ __align__(128) char dyn[];       // ring of chunks; of a teacher's row, per control warp: weights, ids, gradients
-  __shared__ __align__(8) uint64_t bars[2 * PIPE_CHUNKS + 3 * PIPE_ROWS + PIPE_C + 1];
+  extern __shared__ __align__(128) char dyn[];       // ring of chunks; of a teacher's row, per control warp: weights, ids, gradients, table of ids
+  __shared__ __align__(8) uint64_t bars[2 * PIPE_CHUNKS + 3 * PIPE_ROWS + PIPE_C];
   __shared__ float2 part[PIPE_ROWS][PIPE_S + PIPE_G];
   __shared__ __align__(16) float4 xch[PIPE_ROWS][8];
   __shared__ float4 coef[PIPE_ROWS];                 // m, scale, hot: dz = scale exp2((z - m) k) + hot onehot
   __shared__ double acc[PIPE_C][3];
+  __shared__ __align__(16) uint4 lowest;             // a vector of -inf
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, C = q.csize, NCH = q.chunks;
   const int rank = C > 1 ? int(cluster_ctarank()) : 0, cl = int(blockIdx.x) / C, v0 = rank * q.vs;
   const uint32_t full = smem_u32(bars), empty = full + 8 * PIPE_CHUNKS, sdone = empty + 8 * PIPE_CHUNKS, cready = sdone + 8 * PIPE_ROWS,
-                 xbar = cready + 8 * PIPE_ROWS, gdone = xbar + 8 * PIPE_ROWS, gbar = gdone + 8 * PIPE_C;
+                 xbar = cready + 8 * PIPE_ROWS, gdone = xbar + 8 * PIPE_ROWS;
   const float k = MODE == MODE_DISTILL ? LOG2E * a.inv_tau : LOG2E;
-  const int K4 = MODE == MODE_DISTILL ? (a.K + 3) & ~3 : 0;
-  auto entries = [&](int w) { return reinterpret_cast<float*>(dyn + NCH * CHUNK_BYTES) + w * 3 * K4; };
+  const int K4 = MODE == MODE_DISTILL ? (a.K + 3) & ~3 : 0, table = MODE == MODE_DISTILL && GRAD ? top_table(a.K) : 0;
+  auto entries = [&](int w) { return reinterpret_cast<float*>(dyn + NCH * CHUNK_BYTES) + w * (3 * K4 + table); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < PIPE_CHUNKS; ++i) {
@@ -560,8 +582,9 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
       mbar_init(xbar + i * 8, 1);
     }
     for (int i = 0; i < PIPE_C; ++i) mbar_init(gdone + i * 8, PIPE_G);
-    mbar_init(gbar, PIPE_G);
     *abort_flag = 0;
+    const uint32_t inf = ES == 4 ? 0xff800000u : 0xff80ff80u;
+    lowest = make_uint4(inf, inf, inf, inf);
     mbar_fence_init();
   }
   __syncthreads();
@@ -666,13 +689,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
             const uint4* src = reinterpret_cast<const uint4*>(dyn + c.slot * CHUNK_BYTES) + w0;
             float f[LV][N];
 #pragma unroll
-            for (int j = 0; j < LV; ++j) Vec<T>::unpack(src[j * 32], f[j]);
-            if (left_vecs < CHUNK_VECS) {      // the last chunk of a slice: what lies behind it is of other rows
-#pragma unroll
-              for (int j = 0; j < LV; ++j)
-#pragma unroll
-                for (int x = 0; x < N; ++x) f[j][x] = w0 + j * 32 < left_vecs ? f[j][x] : -INFINITY;
-            }
+            for (int j = 0; j < LV; ++j) Vec<T>::unpack(w0 + j * 32 < left_vecs ? src[j * 32] : lowest, f[j]);      // what lies behind a slice is of other rows
             if (!GRAD && h == HALVES - 1) {    // in registers: the chunk is free
               __syncwarp();
               if (lane == 0) mbar_arrive(empty + c.slot * 8);
@@ -732,20 +749,37 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
           tg = tq + 2 * K4;
           if (GRAD && n >= PIPE_C && !(ok = wait(gdone + w * 8, n / PIPE_C - 1, ST_TIMEOUT_TMEM_EMPTY))) break;      // the entries of its last row are written
           float tm = -INFINITY, ts = 0.f, zm = -INFINITY;
-          for (int j = lane; j < K4; j += 32) {
-            const long long y = j < a.K ? ld_idx(a.top_ids, t * a.K + j, a.idx64) : -1;
-            TFB_BOUNDS(y < r.V, 3, y, r.V);
-            bad |= y >= r.V;
-            const bool have = y >= 0 && y < r.V;
-            const float z = have ? ld_z(a.top_z, t * a.K + j, a.top_f32) : -INFINITY;
-            const int g = have ? int((y + s.eoff) / N) - v0 : -1;
-            const bool mine = g >= 0 && g < q.vs;
-            const float zs = mine ? Vec<T>::get(row[y]) : -INFINITY;
-            tid[j] = have ? int(y) : -1;
-            tq[j] = z;
-            tg[j] = zs;
-            if (have) join(tm, ts, z, 1.f, k);
-            zm = fmaxf(zm, zs);
+          // two entries of a lane at a time, since the student's logits can be asked for only when the ids are there.  us at 12500 x 32000, one / two / four: 20 entries 310 / 312 /
+          // 315, 128 360 / 342 / 339, 256 520 / 466 / 425
+          for (int j0 = lane; j0 < K4; j0 += TOP_LOADS * 32) {
+            long long y[TOP_LOADS];
+            float z[TOP_LOADS], zs[TOP_LOADS], mx = tm;
+#pragma unroll
+            for (int u = 0; u < TOP_LOADS; ++u) y[u] = j0 + u * 32 < a.K ? ld_idx(a.top_ids, t * a.K + j0 + u * 32, a.idx64) : -1;
+#pragma unroll
+            for (int u = 0; u < TOP_LOADS; ++u) {
+              TFB_BOUNDS(y[u] < r.V, 3, y[u], r.V);
+              bad |= y[u] >= r.V;
+              if (y[u] < 0 || y[u] >= r.V) y[u] = -1;
+              z[u] = y[u] >= 0 ? ld_z(a.top_z, t * a.K + j0 + u * 32, a.top_f32) : -INFINITY;
+              const int g = y[u] >= 0 ? int((y[u] + s.eoff) / N) - v0 : -1;
+              zs[u] = g >= 0 && g < q.vs ? Vec<T>::get(row[y[u]]) : -INFINITY;
+            }
+#pragma unroll
+            for (int u = 0; u < TOP_LOADS; ++u) {
+              mx = fmaxf(mx, z[u]);
+              zm = fmaxf(zm, zs[u]);
+              if (j0 + u * 32 < K4) {
+                tid[j0 + u * 32] = int(y[u]);
+                tq[j0 + u * 32] = z[u];
+                tg[j0 + u * 32] = zs[u];
+              }
+            }
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            ts *= ex2((tm - ref) * k);
+#pragma unroll
+            for (int u = 0; u < TOP_LOADS; ++u) ts += ex2((z[u] - ref) * k);
+            tm = mx;
           }
           warp_join(tm, ts, k);
           zm = warp_max(zm);
@@ -764,6 +798,37 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
           }
           x1 = warp_sum(x1);
           x2 = warp_sum(x2);
+          if (GRAD) {
+            // the weights of each entry's id, before the row's statistics are there: the ring holds fewer than two rows of 50257, so what comes after them is waited for.
+            // 7959 x 50257 with 64, 256 and 1024 entries: 332, 402 and 1450 us; after the statistics and without the table 357, 738 and 6340.
+            int* seen = tid + 2 * K4;
+            for (int i = lane * 4; i < table; i += 128) *reinterpret_cast<int4*>(seen + i) = make_int4(-1, -1, -1, -1);
+            __syncwarp();
+            bool twice = false;
+            for (int j = lane; j < K4; j += 32) {
+              const int y = tid[j], g = y >= 0 ? int((y + s.eoff) / N) - v0 : -1;
+              if (g < 0 || g >= q.vs) continue;
+              twice |= seen_before(seen, table, y);
+            }
+            if (__any_sync(~0u, twice)) {
+              float* sums_of = reinterpret_cast<float*>(seen);
+              __syncwarp();
+              for (int j = lane; j < K4; j += 32) {
+                float back = 0.f;
+                for (int i = 0; i < K4; i += 4) {
+                  const int4 o = *reinterpret_cast<const int4*>(tid + i);
+                  const float4 u = *reinterpret_cast<const float4*>(tq + i);
+                  back += o.x == tid[j] ? u.x : 0.f;
+                  back += o.y == tid[j] ? u.y : 0.f;
+                  back += o.z == tid[j] ? u.z : 0.f;
+                  back += o.w == tid[j] ? u.w : 0.f;
+                }
+                sums_of[j] = back;
+              }
+              __syncwarp();
+              for (int j = lane; j < K4; j += 32) tq[j] = sums_of[j];
+            }
+          }
         }
         if (!(ok = wait(sdone + rs * 8, use, ST_TIMEOUT_TMEM_FULL))) break;
         const float2 p = lane < SW ? part[rs][lane] : make_float2(-INFINITY, 0.f);
@@ -798,21 +863,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
           }
           if (GRAD) {
             // the entries' own gradients, each from its value of z; the gradient warps store them over what their vectors have written
-            __syncwarp();
-            for (int j = lane; j < K4; j += 32) {
-              const int y = tid[j], g = y >= 0 ? int((y + s.eoff) / N) - v0 : -1;
-              if (g < 0 || g >= q.vs) continue;
-              float back = 0.f;        // an id may come twice
-              for (int i = 0; i < K4; i += 4) {
-                const int4 o = *reinterpret_cast<const int4*>(tid + i);
-                const float4 u = *reinterpret_cast<const float4*>(tq + i);
-                back += o.x == y ? u.x : 0.f;
-                back += o.y == y ? u.y : 0.f;
-                back += o.z == y ? u.z : 0.f;
-                back += o.w == y ? u.w : 0.f;
-              }
-              tg[j] = hot * (ex2((tg[j] - Mr) * k) / S - back);
-            }
+            for (int j = lane; j < K4; j += 32) tg[j] = scale * ex2((tg[j] - Mr) * k) - hot * tq[j];
             __syncwarp();
           }
         } else {
@@ -865,7 +916,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
           for (int v = gw * 32 + lane; v < s.n; v += PIPE_G * 32) store(v0 + v, f);
           continue;
         }
-        const unsigned rs = n % PIPE_ROWS;
+        const unsigned rs = n % PIPE_ROWS, first = c.slot % PIPE_GG;      // group that has the slice's first chunk
         if (!(ok = wait(cready + rs * 8, n / PIPE_ROWS, ST_TIMEOUT_TMEM_FULL))) break;
         const float4 cf = coef[rs];
         const float2 neg = make_float2(-cf.x, -cf.x), k2 = make_float2(k, k), sc = make_float2(cf.y, cf.y);
@@ -917,14 +968,13 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
         }
         if (!ok) break;
         if constexpr (MODE == MODE_DISTILL) {
+          // every warp those of the vectors that it has stored itself
           __syncwarp();
-          if (lane == 0) mbar_arrive(gbar);
-          if (!(ok = wait(gbar, n, ST_TIMEOUT_TMEM_EMPTY))) break;      // every vector of the slice is stored
           const float* tq = entries(n % PIPE_C);
           const int* tid = reinterpret_cast<const int*>(tq + K4);
-          for (int j = gw * 32 + lane; j < K4; j += PIPE_G * 32) {
+          for (int j = lane; j < K4; j += 32) {
             const int yj = tid[j], g = yj >= 0 ? int((yj + s.eoff) / N) - v0 : -1;
-            if (g >= 0 && g < q.vs) out[yj] = Vec<T>::put(tq[2 * K4 + j]);
+            if (g >= 0 && g < q.vs && int((first + g / CHUNK_VECS) % PIPE_GG * PIPE_W + g / (LV * 32) % PIPE_W) == gw) out[yj] = Vec<T>::put(tq[2 * K4 + j]);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(gdone + (n % PIPE_C) * 8);
@@ -1132,7 +1182,7 @@ __global__ void __launch_bounds__(512) pair_kernel(const PairArg a) {
 // The general form's launch.
 template <class T, int MODE>
 static void launch_rows_t(const RowsArg& r, const LossArg& a, bool warp, bool pdl, cudaStream_t st) {
-  const size_t smem = MODE == MODE_DISTILL ? size_t(a.K) * 8 : 0;
+  const size_t smem = MODE == MODE_DISTILL ? size_t(2 * a.K + row_table(warp, a.K)) * 4 : 0;
   if (warp) return tfb::launch_attr(pdl, row_loss_kernel<T, MODE, true>, (r.T + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, smem * WARP_ROWS, st, r, a);
   LossArg q = a;
   if (MODE == MODE_GRAD) {
@@ -1190,7 +1240,7 @@ static int launch_pipe_t(const RowsArg& r, const LossArg& a, PipeArg q, long lon
   // The smallest cluster whose slices are two thirds of the ring, so that the next row's copies go on while a row is finished; larger ones
   // exchange more and leave SMs without a block (33 clusters of 4, 15 of 8, fit on 148 SMs): 3125 x 128256, 4.0 TB/s with 8, 4.9 with 4, 5.0 with 2 (without a gradient
   // 3.2, 4.1, 5.2), 7959 x 50257 3.1 with 4, 4.1 with 2, 5.0 with 1.  Then larger ones while rows are too few to fill the machine.
-  const int extra = MODE == MODE_DISTILL ? PIPE_C * 3 * ((a.K + 3) & ~3) * 4 : 0;
+  const int extra = MODE == MODE_DISTILL ? PIPE_C * (3 * ((a.K + 3) & ~3) + (GRAD ? top_table(a.K) : 0)) * 4 : 0;
   q.chunks = min(PIPE_CHUNKS, (most - extra) / CHUNK_BYTES / (PIPE_SG + PIPE_GG) * (PIPE_SG + PIPE_GG));
   const int slice = q.chunks * 2 / 3 * CHUNK_VECS;
   int C = 1;
