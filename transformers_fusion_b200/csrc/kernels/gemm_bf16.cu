@@ -977,23 +977,24 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
 // -------------------------------------------------------------------------------------------------
 template <bool A_MN, bool B_MN, int BN, bool STATS = false>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const PeerMaps& tpeers, const GemmParams& p,
-                  int grid, cudaStream_t st) {
+                  int grid, cudaStream_t st, bool pdl = pdl_mode() == 2) {
   using L = SmemLayout<BN>;
   static DeviceOnce once;
   auto kern = gemm_bf16_kernel<A_MN, B_MN, BN, STATS>;
   if (int e = ensure_dyn_smem(once, kern, L::TOTAL)) return e;
-  tfb::launch_k(kern, grid, GEMM_THREADS, L::TOTAL, st, ta, tb, tc, tpeers, p);
+  tfb::launch_attr(pdl, kern, grid, GEMM_THREADS, L::TOTAL, st, ta, tb, tc, tpeers, p);
   return int(cudaGetLastError());
 }
 
 template <bool A_MN, bool B_MN, bool STATS = false>
-static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const GemmParams& p, int pairs, cudaStream_t st) {
+static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const GemmParams& p, int pairs, cudaStream_t st,
+                       bool pdl = pdl_mode() == 2) {
   using L = PairSmem;
   static DeviceOnce once;
   static const PeerMaps none = {};
   auto kern = gemm_pair_kernel<A_MN, B_MN, STATS>;
   if (int e = ensure_dyn_smem(once, kern, L::TOTAL)) return e;
-  tfb::launch_k(kern, 2 * pairs, GEMM_THREADS, L::TOTAL, st, ta, tb, tc, none, p);
+  tfb::launch_attr(pdl, kern, 2 * pairs, GEMM_THREADS, L::TOTAL, st, ta, tb, tc, none, p);
   return int(cudaGetLastError());
 }
 
@@ -1446,14 +1447,15 @@ int tfb::gemm_row_stats(const void* A, long long lda, const void* B, long long l
   p.raster_gn = p.tiles_n > 12 && p.tiles_m >= 2 ? 8 : p.tiles_n;
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool pdl = pdl_mode() != 0;      // behind a small kernel whose blocks are all there by then
   int rc;
   if (one) {
     static const PeerMaps none = {};
     if ((rc = make_tmap_3d(&tb, B, 2, K, N, 1, ldb * 2, (unsigned long long)ldb * 2 * N, BK, BM, 1))) return rc;
-    rc = launch<false, false, BM, true>(ta, tb, ta, none, p, int(min(tiles, (long long)sm_count())), st);
+    rc = launch<false, false, BM, true>(ta, tb, ta, none, p, int(min(tiles, (long long)sm_count())), st, pdl);
   } else {
     if ((rc = make_tmap_2d(&tb, B, 2, K, N, ldb * 2, BK, BM))) return rc;
-    rc = launch_pair<false, false, true>(ta, tb, ta, p, int(min(tiles, (long long)sm_count() / 2)), st);
+    rc = launch_pair<false, false, true>(ta, tb, ta, p, int(min(tiles, (long long)sm_count() / 2)), st, pdl);
   }
   return rc ? (rc > 0 ? -1000 - rc : rc) : 2 * p.tiles_n;
 }

@@ -31,7 +31,7 @@ struct ScoreArg {
   long long ignore;
   int M, V, H;
   float *logp, *lse;                   // [M]
-  int* rows;                           // one word, 0 before the launch: rows that are scored
+  int* rows;                           // one word: rows that are scored
   int* row_of;                         // [M]
   __nv_bfloat16* xc;                   // [M, ldc]: their hidden states
   long long ldc;
@@ -42,32 +42,49 @@ struct ScoreArg {
   float* stats;                        // few rows: [2, M]
 };
 
-constexpr int GATHER_ROWS = 8;      // a warp to a row
+constexpr int GATHER_MOST = 1024;    // rows of a block
 
-// Which place a row gets depends on the order in which blocks arrive; what is computed for it does not.
-__global__ void __launch_bounds__(256) score_gather_kernel(const ScoreArg a) {
+// Every block takes `per_block` rows and counts those that are scored before them by itself (the targets of a launch are 256 KB at most), so rows keep
+// their order and no counter has to be cleared by a launch of its own.
+__global__ void __launch_bounds__(1024) score_gather_kernel(const ScoreArg a, const int per_block) {
   tfb::pdl_sync();
-  __shared__ int place[GATHER_ROWS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * GATHER_ROWS;
-  if (warp == 0) {
-    const int row = r0 + lane;
-    const bool mine = lane < GATHER_ROWS && row < a.M, on = mine && ld_idx(a.targets, row, a.idx64) != a.ignore;
-    const unsigned mask = __ballot_sync(~0u, on);
-    int base = 0;
-    if (lane == 0 && mask) base = atomicAdd(a.rows, __popc(mask));
-    base = __shfl_sync(~0u, base, 0);
-    const int at = base + __popc(mask & ((1u << lane) - 1));
-    if (lane < GATHER_ROWS) place[lane] = on ? at : -1;
-    if (on) a.row_of[at] = row;
-    else if (mine) a.logp[row] = a.lse[row] = 0.f;
+  __shared__ int place[GATHER_MOST], sums[32], count[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * per_block, n = min(per_block, a.M - r0);
+  int before = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < r0; i += 1024) before += ld_idx(a.targets, i, a.idx64) != a.ignore;
+  const bool mine = int(threadIdx.x) < n, on = mine && ld_idx(a.targets, r0 + threadIdx.x, a.idx64) != a.ignore;
+  const unsigned mask = __ballot_sync(~0u, on);
+  before = __reduce_add_sync(~0u, before);
+  if (lane == 0) {
+    sums[warp] = before;
+    count[warp] = __popc(mask);
   }
   __syncthreads();
-  const int at = place[warp];
-  if (at < 0) return;
-  const uint4* src = reinterpret_cast<const uint4*>(a.x + (r0 + warp) * a.ldx);
-  uint4* dst = reinterpret_cast<uint4*>(a.xc + at * a.ldc);
-#pragma unroll 8
-  for (int v = lane; v < a.H / 8; v += 32) dst[v] = src[v];
+  const int c = count[lane], all = __reduce_add_sync(~0u, c), base = __reduce_add_sync(~0u, sums[lane]);
+  const int at = base + __reduce_add_sync(~0u, lane < warp ? c : 0) + __popc(mask & ((1u << lane) - 1));
+  if (mine) {
+    place[threadIdx.x] = on ? at : -1;
+    if (on) a.row_of[at] = r0 + threadIdx.x;
+    else a.logp[r0 + threadIdx.x] = a.lse[r0 + threadIdx.x] = 0.f;
+  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.rows = base + all;
+  __syncthreads();
+  // a warp takes pieces of a row, four vectors to a lane
+  const int vecs = a.H / 8, pieces = (vecs + 127) / 128;
+  for (int i = warp; i < n * pieces; i += 32) {
+    const int row = i / pieces, v = (i - row * pieces) * 128 + lane, to = place[row];
+    if (to < 0) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(a.x + (r0 + row) * a.ldx) + v;
+    uint4* dst = reinterpret_cast<uint4*>(a.xc + to * a.ldc) + v;
+    uint4 w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (v + u * 32 < vecs) w[u] = src[u * 32];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (v + u * 32 < vecs) dst[u * 32] = w[u];
+  }
 }
 
 // A thread's share of x[row] . w[target]; NaN for a target outside the vocabulary.
@@ -187,11 +204,11 @@ TFB_API int tfb_linear_logprobs(const ScoreArg* p, int* status, void* stream) {
       return int(cudaGetLastError());
     }
   }
-  if (cudaError_t e = cudaMemsetAsync(p->rows, 0, sizeof(int), st)) return int(e);
-  tfb::launch_k(score_gather_kernel, (p->M + GATHER_ROWS - 1) / GATHER_ROWS, 256, 0, st, *p);
+  const int blocks = max(sm_count(), (p->M + GATHER_MOST - 1) / GATHER_MOST), per_block = (p->M + blocks - 1) / blocks;
+  tfb::launch_k(score_gather_kernel, (p->M + per_block - 1) / per_block, 1024, 0, st, *p, per_block);
   ScoreArg a = *p;
   a.parts = gemm_row_stats(p->xc, p->ldc, p->w, p->ldw, p->M, p->V, p->H, p->rows, p->part, status, stream);
   if (a.parts <= 0) return a.parts <= -1000 ? -1000 - a.parts : a.parts;
-  tfb::launch_k(score_finish_kernel, (p->M + 7) / 8, 256, 0, st, a);
+  tfb::launch_k_pdl(score_finish_kernel, (p->M + 7) / 8, 256, 0, st, a);
   return int(cudaGetLastError());
 }
