@@ -199,6 +199,34 @@ def test_logits_that_the_backward_pass_reads_stay(dev):
     same(got, want * (1 - 0.01 * 0.04), dev)
 
 
+class Capped(DenseModel):
+    """A model of the framework's class with a forward pass of its own, whose backward reads the logits that it returned."""
+
+    def forward(self, ids):
+        return torch.tanh(super().forward(ids))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["forward", "hook"])
+def test_forward_passes_of_other_kinds_keep_their_logits(dev, kind):
+    cfg = model("cpu").cfg
+    m = (Capped if kind == "forward" else DenseModel)(cfg, device=dev, dtype=torch.float32 if dev == "cpu" else torch.bfloat16, seed=0)
+    seen = []
+    if kind == "hook":
+        m.register_forward_hook(lambda mod, args, out: seen.append((out.detach(), out.detach().clone())))
+    t = rl.GRPOTrainer(m, group_size=4, beta=0.0, clip_eps=0.0)
+    ids, mask, g = batch(dev)
+    rewards = torch.tensor([1.0, 0.2, -0.5, 0.7])
+    got, loss = stepped_gradients(t, lambda: t.train_step(ids, mask, rewards))
+    adv, w = t.advantages(rewards).to(dev)[:, None], mask[:, 1:]
+    want, wloss = plain_gradients(m, lambda: -(((adv * lp64(m, ids)) * w).sum(-1) / w.sum(-1).clamp(min=1)).mean())
+    same(got, want, dev)
+    assert all(torch.equal(a, b) for a, b in seen)
+    # and are scored as they are
+    lp = torch.log_softmax(m(ids[:1, :9]).float(), -1)[0, 4:8].gather(-1, ids[0, 5:9, None]).mean()
+    assert abs(ED.EvalHarness(m)._seq_logp(ids[0, :5].tolist(), ids[0, 5:9].tolist()) - lp.item()) <= 1e-5 * abs(lp.item())
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_score_tokens(dev):
     m = model(dev)

@@ -15,6 +15,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as TF
 
+from ..models.dense import ends_in_head
 from ..ops import losses as L
 from ..trainer import training_utils as TU
 from ..trainer.optimizers import build_optimizer
@@ -674,7 +675,7 @@ class EvalHarness:
         at = slice(len(ctx) - 1, len(ctx) + len(cont) - 1)
         targets = torch.full_like(ids, -100)
         targets[0, at] = ids[0, len(ctx):]
-        score = getattr(self.model, "score_tokens", None) or (lambda ids, targets: L.token_logprobs(self.model(ids).float(), targets))
+        score = self.model.score_tokens if ends_in_head(self.model) else lambda ids, targets: L.token_logprobs(self.model(ids).float(), targets)
         with torch.no_grad():
             return float(score(ids, targets)[0, at].mean())
 

@@ -571,6 +571,13 @@ class _FinalNormFn(torch.autograd.Function):
         return _norm_bwd(m.cfg, dy.contiguous(), ctx.h, m.norm, m.norm_bias, ctx.st, None), None, None
 
 
+def ends_in_head(model) -> bool:
+    """Whether ``model(ids)`` is the forward pass of ``DenseModel`` and nothing sees or changes the logits that it returns (another forward pass, hooks): they are
+    the head's product with ``hidden_states`` then, and nobody else's."""
+    return (isinstance(model, DenseModel) and type(model).forward is DenseModel.forward and "forward" not in vars(model)
+            and not model._forward_hooks and not torch.nn.modules.module._global_forward_hooks)
+
+
 class _LinearFn(torch.autograd.Function):
     """y = x W^T with the weight gradient accumulated into W.main_grad."""
 

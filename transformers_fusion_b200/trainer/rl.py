@@ -25,6 +25,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as TF
 
+from ..models.dense import ends_in_head
 from ..ops import losses as L
 from .fused_optim import FlatAdamW
 
@@ -69,11 +70,12 @@ class _RLBase:
         self.steps = 0
 
     def _forward(self, ids):
-        """(logits with their graph, the same values without it, where their gradient may go).  The models here end in a linear head, whose backward does
-        not read what it returned: the gradient then takes the logits' place.  Another model's logits are left as they are."""
+        """(logits with their graph, the same values without it, where their gradient may go).  The forward pass of the models here ends in a linear head, whose
+        backward does not read what it returned: the gradient then takes the logits' place.  The logits of another forward pass, and of a model whose hooks
+        may have kept them, are left as they are."""
         logits = _loss_logits(self.model(ids))
         z = logits.detach()
-        return logits, z, z if hasattr(self.model, "score_tokens") else None
+        return logits, z, z if ends_in_head(self.model) else None
 
     def _backward_and_step(self, logits, dlogits, grad_scale=1.0):
         logits.backward(dlogits)
