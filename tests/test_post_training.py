@@ -3,12 +3,15 @@ operators one after the other as a training run uses them, and scoring without l
 
 The gradients of a whole model are compared in fp32 on the CPU (two orders of the same 32-bit sums: 1e-5 of the largest entry), and on the GPU, where model and gradient are
 bfloat16, by the angle between them: every logit gradient is rounded to 2^-9 of itself in both, at different places, as are the products behind it."""
+import threading
+
 import pytest
 import torch
 
 from transformers_fusion_b200.engines import dense as ED
 from transformers_fusion_b200.models.config import TransformerConfig
 from transformers_fusion_b200.models.dense import DenseModel
+from transformers_fusion_b200.ops import functional as F
 from transformers_fusion_b200.ops import losses as L
 from transformers_fusion_b200.trainer import rl
 
@@ -199,6 +202,28 @@ def test_logits_that_the_backward_pass_reads_stay(dev):
     same(got, want * (1 - 0.01 * 0.04), dev)
 
 
+@pytest.mark.gpu
+def test_first_work_of_a_thread():
+    """A product is the first GPU work of a new thread, as of autograd's when the logits' gradient is handed to it."""
+    x = torch.randn(192, 256, device="cuda").bfloat16()
+    w = torch.randn(320, 256, device="cuda").bfloat16()
+    out, errors = torch.zeros(192, 320, device="cuda", dtype=torch.bfloat16), []
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            F.gemm(x, w, out=out)
+        except Exception as e:      # the thread's own
+            errors.append(e)
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    want = x.double() @ w.double().t()
+    assert ((out.double() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -20 * (x.double().abs() @ w.double().abs().t())).all()
+
+
 class Capped(DenseModel):
     """A model of the framework's class with a forward pass of its own, whose backward reads the logits that it returned."""
 
@@ -222,8 +247,9 @@ def test_forward_passes_of_other_kinds_keep_their_logits(dev, kind):
     want, wloss = plain_gradients(m, lambda: -(((adv * lp64(m, ids)) * w).sum(-1) / w.sum(-1).clamp(min=1)).mean())
     same(got, want, dev)
     assert all(torch.equal(a, b) for a, b in seen)
-    # and are scored as they are
-    lp = torch.log_softmax(m(ids[:1, :9]).float(), -1)[0, 4:8].gather(-1, ids[0, 5:9, None]).mean()
+    # and are scored as they are (by a pass without a graph, which rounds at other places)
+    with torch.no_grad():
+        lp = torch.log_softmax(m(ids[:1, :9]).float(), -1)[0, 4:8].gather(-1, ids[0, 5:9, None]).mean()
     assert abs(ED.EvalHarness(m)._seq_logp(ids[0, :5].tolist(), ids[0, 5:9].tolist()) - lp.item()) <= 1e-5 * abs(lp.item())
 
 

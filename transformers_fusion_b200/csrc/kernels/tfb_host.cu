@@ -20,6 +20,16 @@ static void load_encode() {
   }
 }
 
+// The driver's call wants a current context, and a thread has none before its first runtime call that makes one so: the thread of autograd whose
+// first work is one of these kernels.  cudaSetDevice does (and is allowed under stream capture).
+template <class F>
+static int with_context(F encode) {
+  if (encode() == CUDA_SUCCESS) return TFB_OK;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return TFB_ERR_DRIVER;
+  return encode() == CUDA_SUCCESS ? TFB_OK : TFB_ERR_DRIVER;
+}
+
 static CUtensorMapDataType dtype_of(int elem_bytes) {
   switch (elem_bytes) {
     case 1: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -37,11 +47,10 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t in
   cuuint64_t strides[1] = {ld_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(out, dtype_of(elem_bytes), 2, const_cast<void*>(base), dims, strides, box, estr,
+  return with_context([&] { return g_encode(out, dtype_of(elem_bytes), 2, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? TFB_OK : TFB_ERR_DRIVER;
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); });
 }
 
 int make_tmap_3d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t d0, uint64_t d1, uint64_t d2,
@@ -53,11 +62,10 @@ int make_tmap_3d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t d0
   cuuint64_t strides[2] = {s1_bytes, s2_bytes};
   cuuint32_t box[3] = {b0, b1, b2};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(out, dtype_of(elem_bytes), 3, const_cast<void*>(base), dims, strides, box, estr,
+  return with_context([&] { return g_encode(out, dtype_of(elem_bytes), 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? TFB_OK : TFB_ERR_DRIVER;
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); });
 }
 
 int make_tmap_4d(CUtensorMap* out, const void* base, int elem_bytes, const uint64_t (&dims)[4], const uint64_t (&strides_bytes)[3],
@@ -70,10 +78,9 @@ int make_tmap_4d(CUtensorMap* out, const void* base, int elem_bytes, const uint6
   cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
   for (int i = 0; i < 4; ++i) { d[i] = dims[i]; b[i] = box[i]; }
   for (int i = 0; i < 3; ++i) s[i] = strides_bytes[i];
-  CUresult r = g_encode(out, dtype_of(elem_bytes), 4, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return with_context([&] { return g_encode(out, dtype_of(elem_bytes), 4, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? TFB_OK : TFB_ERR_DRIVER;
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); });
 }
 
 int pdl_mode() {
