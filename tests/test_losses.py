@@ -662,3 +662,36 @@ def test_repeats_bit_for_bit(V, T):
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
     _lib.check_status()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,apart", [(40, False), (20001, False), (20001, True)], ids=["warp", "pipeline", "block"])
+@pytest.mark.parametrize("kw", [dict(), dict(mean="sum"), dict(ref=True), dict(ref=True, kl_coef=0.1)], ids=["clip", "sum", "reported", "kl"])
+def test_bad_rows_of_a_clipped_policy(dev, dtype, V, apart, kw):
+    """On the policy's own tokens the ratio is 1 whatever their log-probability is, but a row that has none (a NaN, an infinity, nothing left by the mask, a target that is masked
+    or outside the vocabulary) makes the loss NaN, as its gradient is; the other rows keep theirs."""
+    kw = dict(kw)
+    z, y = make("cpu", (3,), V, dtype, V, ignored=0.0)
+    ref = torch.full((3,), -2.0, device=dev) if kw.pop("ref", False) else None
+    A = torch.tensor([0.7, -0.4, 0.2], device=dev)
+
+    def call(z, y):
+        z, y = z.to(dev), y.to(dev)
+        out = torch.empty(3 * V + 1, dtype=dtype, device=dev)[1:].view(3, V) if apart else None      # rows that start elsewhere in a vector
+        return L.policy_loss_fwd_bwd(z, y, A, None, ref, out=out, **kw)
+    good = call(z, y)
+    assert good.loss.isfinite() and good.dlogits.isfinite().all()
+    for kind in ("nan", "inf", "empty", "outside", "before", "masked"):
+        b, t = z.clone(), y.clone()
+        if kind in ("nan", "inf"):
+            b[1, (t[1] + 1) % V] = math.nan if kind == "nan" else math.inf
+        elif kind == "empty":
+            b[1] = -math.inf
+        elif kind == "masked":
+            b[1, t[1]] = -math.inf
+        else:
+            t[1] = V if kind == "outside" else -3
+        o = call(b, t)
+        assert o.loss.isnan() and o.dlogits[1].isnan().all(), kind
+        assert torch.equal(o.dlogits[[0, 2]], good.dlogits[[0, 2]]), kind

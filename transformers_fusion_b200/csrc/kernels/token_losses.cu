@@ -126,6 +126,7 @@ __device__ __forceinline__ float weight_of(const LossArg& a, long long t, int S)
 
 // The policy's term of one token: l, its KL estimate, whether the clip took its gradient, and g = dl / dlp.
 //   s = r A, r = exp(lp - old); with a clip the smaller of that and clamp(r) A, whose gradient is 0 where it is the smaller one.
+//   Without older log-probabilities old is lp itself, so that a row without a log-probability (NaN, -inf) has no ratio either: its loss is NaN as its gradient is.
 //   Without a ratio s = A lp.  kl: k3 = exp(x) - 1 - x, k1 = x, x = ref - lp.
 __device__ __forceinline__ void policy_terms(const LossArg& a, float lp, float lp_old, float ref_lp, float A, float& l, float& kl, float& clipped, float& g) {
   float s, ds;
@@ -152,7 +153,7 @@ __device__ __forceinline__ void policy_terms(const LossArg& a, float lp, float l
 }
 
 __device__ __forceinline__ void policy_row(const LossArg& a, double lp, long long t, long long b, float& l, float& kl, float& clipped, float& g) {
-  policy_terms(a, float(lp), a.old_lp ? float(lp - double(a.old_lp[t])) : 0.f, a.ref_lp ? float(double(a.ref_lp[t]) - lp) : 0.f, a.adv[a.adv_seq ? b : t], l, kl,
+  policy_terms(a, float(lp), float(lp - (a.old_lp ? double(a.old_lp[t]) : lp)), a.ref_lp ? float(double(a.ref_lp[t]) - lp) : 0.f, a.adv[a.adv_seq ? b : t], l, kl,
                clipped, g);
 }
 
@@ -872,7 +873,8 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
           if (rank == 0 && lane == 0) put_stats<MODE>(a, r.T, t, M, ls, lp);
           if constexpr (MODE == MODE_POLICY) {
             float loss, kl, clipped, g;
-            policy_terms(a, float(lp), a.old_lp ? float(lp - double(__shfl_sync(~0u, old_lp, l))) : 0.f,
+            const double from = a.old_lp ? double(__shfl_sync(~0u, old_lp, l)) : lp;
+            policy_terms(a, float(lp), float(lp - from),
                          a.ref_lp ? float(double(__shfl_sync(~0u, ref_lp, l)) - lp) : 0.f, __shfl_sync(~0u, adv, l), loss, kl, clipped, g);
             hot = wrow * g;
             scale = -hot / S;
