@@ -695,3 +695,28 @@ def test_bad_rows_of_a_clipped_policy(dev, dtype, V, apart, kw):
         o = call(b, t)
         assert o.loss.isnan() and o.dlogits[1].isnan().all(), kind
         assert torch.equal(o.dlogits[[0, 2]], good.dlogits[[0, 2]]), kind
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M,H,V", [(1, 64, 300), (7, 72, 1), (9, 512, 4000), (61, 1024, 50257), (65, 256, 1001), (100, 512, 32000), (100, 2048, 4001), (128, 1024, 777), (129, 64, 260),
+                                   (300, 256, 1001), (1500, 512, 8000)])
+def test_scoring_of_nearly_certain_tokens(dev, M, H, V):
+    """Targets whose probability is 0.5 to 1 - 1e-12.  With e the errors of the products (each H 2^-24 of the sum of its terms' sizes at most) lp is off by (1 - p) times two of them,
+    by REL of 1 - p from the statistics, and by its own rounding: what a nearly certain token's is off by shrinks with it, down to what 64 bits hold next to 1 (2^-53 a sum, 2^-44 in all)."""
+    g = gen("cpu", H + V)
+    w = (torch.randn(V, H, generator=g) * 2 / math.sqrt(H)).to(BF)
+    y = torch.randint(0, V, (M,), generator=g)
+    x = (w[y].float() * (10 + 30 * torch.rand(M, 1, generator=g)) / 4).to(BF)
+    y[torch.rand(M, generator=g) < 0.2] = IGN
+    x, w, y = x.to(dev), w.to(dev), y.to(dev)
+    keep = y != IGN
+    z = x.double() @ w.double().t()
+    zy = z.gather(1, y.clamp(min=0)[:, None])
+    others = torch.logsumexp(z.scatter(1, y.clamp(min=0)[:, None], -math.inf), 1) - zy[:, 0]      # log((1 - p) / p)
+    lp, q = -torch.nn.functional.softplus(others) * keep, torch.sigmoid(others)
+    size = (x.double().abs() @ w.double().abs().t()).max(1).values
+    tol = q * (2 * H * 2 ** -24 * size + REL) + 2 ** -23 * lp.abs() + 2 ** -44
+    got, lse = L.linear_logprobs(x, w, y)
+    near(got, lp, tol * keep, "logp")
+    near(lse, torch.logsumexp(z, 1) * keep, (H * 2 ** -24 * size + REL / 2 + 2 ** -23 * z.abs().max(1).values) * keep, "lse")
+    assert (got <= 0).all()

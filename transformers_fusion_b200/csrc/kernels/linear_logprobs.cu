@@ -1,27 +1,19 @@
 // Log-probabilities of given tokens under a head, from hidden states: lp = x . w[y] - log sum_v exp(x . w[v]), without the [T, V] logits in memory.
 //
 //   gather   rows that are scored, one behind the other: a prompt's rows take no part in the product
-//   product  x W^T on tensor cores (gemm_bf16.cu), whose epilogue keeps (m, sum exp) of every row's columns in half a tile and drops the rest
-//   finish   joins a row's parts (or takes its statistics), and takes the product with its target's row of W by itself, in 32-bit fused multiply-adds: the tensor cores'
-//            accumulation is off by a few 2^-24 of the partial sums at each of its steps, in one direction, which the log of a sum over
-//            thousands of columns does not show but the one value that is subtracted from it does (relative error of lp at 4096 terms 1.3e-6 against 2.6e-7)
+//   product  x W^T on tensor cores (gemm_bf16.cu), whose epilogue keeps (m, sum exp) of every row's columns in half a tile, the target's left out, and drops the rest
+//   finish   joins a row's parts, takes the product with its target's row of W by itself, in 32-bit fused multiply-adds, and puts the two together
+//
+// The target's column is left out of the sum because its logit there is another rounding of the same number: the tensor cores' accumulation is off by a few 2^-24 of the
+// partial sums at each of its steps, in one direction (relative error of lp at 4096 terms 1.3e-6 with their value, 2.6e-7 with the multiply-adds').  Where the
+// target is most of the sum the difference of the two would be all of lp; so it is the other columns' share that lp is computed from (score_of).
+// Few rows (see below) are not gathered: their logits, the rows that are not scored among them, stand in a workspace.
+#include "row_losses.cuh"
 #include "tfb_host.h"
-#include "tfb_ptx.cuh"
 
 TFB_BOUNDS_DEFINE(linear_logprobs)
 
 namespace tfb {
-
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ long long ld_idx(const void* p, long long i, int is64) {
-  return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
-}
 
 struct ScoreArg {
   const __nv_bfloat16 *x, *w;
@@ -32,14 +24,14 @@ struct ScoreArg {
   int M, V, H;
   float *logp, *lse;                   // [M]
   int* rows;                           // one word: rows that are scored
-  int* row_of;                         // [M]
+  int *row_of, *col_of;                // [M]: place of a scored row, and its target (-1 outside the vocabulary)
   __nv_bfloat16* xc;                   // [M, ldc]: their hidden states
   long long ldc;
   float2* part;                        // [2 ceil(V / 128), M]
   int parts;                           // of a row; set by the launch
   float* z;                            // few rows, else null: [M, ldz] logits, ldz a multiple of 4
   long long ldz;
-  float* stats;                        // few rows: [2, M]
+  float* zy;                           // few rows: [M] the targets' logits
 };
 
 constexpr int GATHER_MOST = 1024;    // rows of a block
@@ -53,7 +45,9 @@ __global__ void __launch_bounds__(1024) score_gather_kernel(const ScoreArg a, co
   int before = 0;
 #pragma unroll 8
   for (int i = threadIdx.x; i < r0; i += 1024) before += ld_idx(a.targets, i, a.idx64) != a.ignore;
-  const bool mine = int(threadIdx.x) < n, on = mine && ld_idx(a.targets, r0 + threadIdx.x, a.idx64) != a.ignore;
+  const bool mine = int(threadIdx.x) < n;
+  const long long y = mine ? ld_idx(a.targets, r0 + threadIdx.x, a.idx64) : a.ignore;
+  const bool on = y != a.ignore;
   const unsigned mask = __ballot_sync(~0u, on);
   before = __reduce_add_sync(~0u, before);
   if (lane == 0) {
@@ -65,8 +59,12 @@ __global__ void __launch_bounds__(1024) score_gather_kernel(const ScoreArg a, co
   const int at = base + __reduce_add_sync(~0u, lane < warp ? c : 0) + __popc(mask & ((1u << lane) - 1));
   if (mine) {
     place[threadIdx.x] = on ? at : -1;
-    if (on) a.row_of[at] = r0 + threadIdx.x;
-    else a.logp[r0 + threadIdx.x] = a.lse[r0 + threadIdx.x] = 0.f;
+    if (on) {
+      a.row_of[at] = r0 + threadIdx.x;
+      a.col_of[at] = y >= 0 && y < a.V ? int(y) : -1;
+    } else {
+      a.logp[r0 + threadIdx.x] = a.lse[r0 + threadIdx.x] = 0.f;
+    }
   }
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.rows = base + all;
   __syncthreads();
@@ -87,12 +85,8 @@ __global__ void __launch_bounds__(1024) score_gather_kernel(const ScoreArg a, co
   }
 }
 
-// A thread's share of x[row] . w[target]; NaN for a target outside the vocabulary.
-__device__ __forceinline__ float target_logit(const ScoreArg& a, long long row, int tid, int nt) {
-  const long long y = ld_idx(a.targets, row, a.idx64);
-  const bool in = y >= 0 && y < a.V;
-  if (tid == 0) TFB_BOUNDS(in, 3, y, a.V);
-  if (!in) return NAN;
+// A thread's share of x[row] . w[y], y in the vocabulary.
+__device__ __forceinline__ float target_logit(const ScoreArg& a, long long row, long long y, int tid, int nt) {
   const uint4 *p = reinterpret_cast<const uint4*>(a.x + row * a.ldx), *q = reinterpret_cast<const uint4*>(a.w + y * a.ldw);
   float2 t = make_float2(0.f, 0.f), u = t;
 #pragma unroll 8
@@ -104,11 +98,6 @@ __device__ __forceinline__ float target_logit(const ScoreArg& a, long long row, 
     u = fma2(unpack_bf16(f.w), unpack_bf16(g.w), u);
   }
   return (t.x + u.x) + (t.y + u.y);
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
 }
 
 // Eight rows to a block (two sectors of a part's entries), 32 threads to a row's parts with eight loads under way in each: a row of a vocabulary of 128256 has 1002 or 2004
@@ -140,8 +129,9 @@ __global__ void __launch_bounds__(256) score_finish_kernel(const ScoreArg a) {
     sh[share][i] = make_float2(m, s);
   }
   for (int i = warp; i < R && r0 + i < n; i += 8) {
-    const int row = a.row_of[r0 + i];
-    const float z = warp_sum(target_logit(a, row, lane, 32));
+    const int y = a.col_of[r0 + i], row = a.row_of[r0 + i];
+    if (lane == 0) TFB_BOUNDS(y >= 0, 3, y, a.V);
+    const float z = y >= 0 ? warp_sum(target_logit(a, row, y, lane, 32)) : 0.f;
     if (lane == 0) zy[i] = z;
   }
   __syncthreads();
@@ -157,26 +147,27 @@ __global__ void __launch_bounds__(256) score_finish_kernel(const ScoreArg a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (lane) continue;
-    const double ls = log(s), lp = double(zy[i]) - double(m) - ls;
     const int row = a.row_of[r0 + i];
-    a.lse[row] = float(double(m) + ls);
-    a.logp[row] = lp > 0.0 ? 0.f : float(lp);      // the two products' roundings are not the same
+    score_of(m, s, zy[i], a.col_of[r0 + i] >= 0, a.logp[row], a.lse[row]);
   }
 }
 
-// The same for rows whose statistics are there: a block to a row.
-__global__ void __launch_bounds__(128) score_rows_kernel(const ScoreArg a) {
+// Few rows, whose logits are there: the target's own, and its column out of the row's statistics.  A block to a row.
+__global__ void __launch_bounds__(128) score_target_kernel(const ScoreArg a) {
   tfb::pdl_sync();
   __shared__ float sh[4];
   const int row = blockIdx.x;
-  const bool on = ld_idx(a.targets, row, a.idx64) != a.ignore;
-  const float z = on ? warp_sum(target_logit(a, row, threadIdx.x, 128)) : 0.f;
+  const long long y = ld_idx(a.targets, row, a.idx64);
+  if (y == a.ignore) return;
+  const bool in = y >= 0 && y < a.V;
+  if (threadIdx.x == 0) TFB_BOUNDS(in, 3, y, a.V);
+  if (!in) return;
+  const float z = warp_sum(target_logit(a, row, y, threadIdx.x, 128));
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = z;
   __syncthreads();
   if (threadIdx.x) return;
-  const double m = a.stats[row], ls = a.stats[a.M + row], lp = double((sh[0] + sh[1]) + (sh[2] + sh[3])) - m - ls;
-  a.lse[row] = float(m + ls);
-  a.logp[row] = lp > 0.0 ? 0.f : float(lp);
+  a.zy[row] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  a.z[row * a.ldz + y] = -INFINITY;
 }
 
 }  // namespace tfb
@@ -185,7 +176,7 @@ using namespace tfb;
 
 // x [M, H] and w [V, H] bf16, pitches multiples of 8, 16-byte aligned; H a multiple of 8.  Writes all of the workspace that it reads.
 TFB_API int tfb_linear_logprobs(const ScoreArg* p, int* status, void* stream) {
-  if (!p || !p->x || !p->w || !p->targets || !p->logp || !p->lse || !p->rows || !p->row_of || !p->xc || !p->part || p->M <= 0 || p->V <= 0 || p->H <= 0 || p->H % 8 ||
+  if (!p || !p->x || !p->w || !p->targets || !p->logp || !p->lse || !p->rows || !p->row_of || !p->col_of || !p->xc || !p->part || p->M <= 0 || p->V <= 0 || p->H <= 0 || p->H % 8 ||
       p->ldx % 8 || p->ldw % 8 || p->ldc % 8 || ((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->w) | reinterpret_cast<uintptr_t>(p->xc)) & 15))
     return TFB_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -193,21 +184,20 @@ TFB_API int tfb_linear_logprobs(const ScoreArg* p, int* status, void* stream) {
   // too few rows high to keep enough of W under way), and the logits stay in L2.  us, this way / that kernel, rows x V x H: 1 x 128256 x 4096 165 / 298, 61 x 128256 x 4096
   // 183 / 216, 128 x 128256 x 4096 213 / 222, 61 x 32000 x 512 21.2 / 23.4, but 128 x 32000 x 512 28 / 21 and 128 x 128256 x 512 71 / 45.
   if (p->z && (p->M <= 64 || (p->M <= 128 && p->H >= 2048))) {
-    if (!p->stats || p->ldz % 4 || (reinterpret_cast<uintptr_t>(p->z) & 15)) return TFB_ERR_ARG;
+    if (!p->zy || p->ldz % 4 || (reinterpret_cast<uintptr_t>(p->z) & 15)) return TFB_ERR_ARG;
     int rc = gemm_skinny(p->x, p->ldx, p->w, p->ldw, p->z, p->ldz, p->M, p->V, p->H, nullptr, nullptr, 0, 1.f, 0, 1, stream);
     if (rc == TFB_NOT_TAKEN)
       rc = gemm_rows(p->x, p->ldx, p->w, p->ldw, nullptr, nullptr, -1, 0, p->z, p->ldz, p->M, p->V, p->H, p->H, nullptr, nullptr, 0, 1.f, 0, 1, 0, status, stream);
     if (rc != TFB_NOT_TAKEN) {
-      if (!rc) rc = row_stats(p->z, p->ldz, p->M, p->V, p->targets, p->idx64, p->ignore, p->stats, status, stream);
       if (rc) return rc;
-      tfb::launch_k_pdl(score_rows_kernel, p->M, 128, 0, st, *p);
-      return int(cudaGetLastError());
+      tfb::launch_k_pdl(score_target_kernel, p->M, 128, 0, st, *p);
+      return row_scores(p->z, p->ldz, p->M, p->V, p->targets, p->idx64, p->ignore, p->zy, p->logp, p->lse, status, stream);
     }
   }
   const int blocks = max(sm_count(), (p->M + GATHER_MOST - 1) / GATHER_MOST), per_block = (p->M + blocks - 1) / blocks;
   tfb::launch_k(score_gather_kernel, (p->M + per_block - 1) / per_block, 1024, 0, st, *p, per_block);
   ScoreArg a = *p;
-  a.parts = gemm_row_stats(p->xc, p->ldc, p->w, p->ldw, p->M, p->V, p->H, p->rows, p->part, status, stream);
+  a.parts = gemm_row_stats(p->xc, p->ldc, p->w, p->ldw, p->M, p->V, p->H, p->rows, p->col_of, p->part, status, stream);
   if (a.parts <= 0) return a.parts <= -1000 ? -1000 - a.parts : a.parts;
   tfb::launch_k_pdl(score_finish_kernel, (p->M + 7) / 8, 256, 0, st, a);
   return int(cudaGetLastError());

@@ -57,12 +57,15 @@ int gemm_rows_glu(const void* x, long long ldx, const void* W, long long ldw, vo
                   int* status, void* stream);
 int gemm_skinny_glu(const void* x, long long ldx, const void* W, long long ldw, void* C, long long ldc, int M, int F, int K, int act, void* stream);
 
-// gemm_bf16.cu: (maximum, sum of exponentials) of the rows of A . B^T, in parts of their columns.  Returns the number of parts, a tfb error, or
-// -1000 - a cudaError_t.
-int gemm_row_stats(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const int* rows, float2* part, int* status, void* stream);
+// gemm_bf16.cu: (maximum, sum of exponentials) of the rows of A . B^T, in parts of their columns and without the column skip[row] (-1: none).  Returns the
+// number of parts, a tfb error, or -1000 - a cudaError_t.
+int gemm_row_stats(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const int* rows, const int* skip, float2* part, int* status,
+                   void* stream);
 
-// token_losses.cu: maximum and log of the sum of exponentials of fp32 rows, stats [2, T]; 0 where the target is `ignore`
-int row_stats(const float* z, long long ldz, int T, int V, const void* targets, int idx64, long long ignore, float* stats, int* status, void* stream);
+// token_losses.cu: log-probabilities of the targets and logsumexp of fp32 rows, whose targets' columns hold -inf and whose targets' logits are in zy [T]; 0
+// where the target is `ignore`
+int row_scores(const float* z, long long ldz, int T, int V, const void* targets, int idx64, long long ignore, const float* zy, float* logp, float* lse, int* status,
+               void* stream);
 
 // Launch of a kernel of this library: same meaning as kernel<<<grid, block, smem, stream>>>(args...), plus the launch
 // attribute that lets the kernel's CTAs be placed while the previous kernel of the stream drains (each kernel starts with

@@ -8,21 +8,14 @@
 // margin is the difference of two sums over a thousand tokens.  The gradient is rounded once, to the type of the logits.
 //
 // Reference counterparts: token log-probs, ratio clipping and KL of the RL trainers (src/trainer/trainer_rl.cpp:557-1350).
+#include "row_losses.cuh"
 #include "tfb_host.h"
-#include "tfb_ptx.cuh"
 
 TFB_BOUNDS_DEFINE(token_losses)
 
 namespace tfb {
 
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TL_MAX_TOP = 1024;      // entries of a teacher's row
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Rows of logits and of their gradient: row t is position t % S of sequence t / S.  Strides in elements; the last dimension is dense.
 struct RowsArg {
@@ -33,7 +26,7 @@ struct RowsArg {
   int* status;                         // device status word of the bounded waits
 };
 
-enum : int { MODE_STATS = 0, MODE_GRAD = 1, MODE_POLICY = 2, MODE_DISTILL = 3 };
+enum : int { MODE_STATS = 0, MODE_GRAD = 1, MODE_POLICY = 2, MODE_DISTILL = 3, MODE_SCORE = 4 };
 enum : int { KL_K3 = 0, KL_K1 = 1 };
 enum : int { MEAN_TOKENS = 0, MEAN_SEQUENCES = 1, MEAN_SUM = 2 };
 
@@ -45,6 +38,9 @@ struct LossArg {
   float* logp;                         // [T]
   float* stats;                        // [2, T]: m and log S apart, since their sum in 32 bits loses log S where |m| is large; MODE_GRAD reads them
   double* logp64;                      // [T], preference
+  // MODE_SCORE: rows without their targets' columns, which are -inf in z
+  const float* zy;                     // [T] the targets' logits
+  float* lse;                          // [T]
   // MODE_GRAD: coefficient of a row
   const float* dlogp;                  // [T], or [T / S] with per_seq
   int per_seq, split;                  // blocks of a row
@@ -63,10 +59,6 @@ struct LossArg {
   float* terms;                        // general form, [3, T]: weighted loss, kl, share of clipped tokens
   int* zero;                           // a word that the first block clears for the kernel that follows, or null
 };
-
-__device__ __forceinline__ long long ld_idx(const void* p, long long i, int is64) {
-  return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
-}
 
 __device__ __forceinline__ float ld_z(const void* row, long long i, int f32) {
   return f32 ? static_cast<const float*>(row)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
@@ -100,11 +92,6 @@ __device__ __forceinline__ float warp_max(float v) {
   float m;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
 }
 // (m, s) of all lanes together, the same bits in every lane
 __device__ __forceinline__ void warp_join(float& m, float& s, float k) {
@@ -157,16 +144,21 @@ __device__ __forceinline__ void policy_row(const LossArg& a, double lp, long lon
                clipped, g);
 }
 
-// what a row leaves behind: m, log S and the log-probability of its target
+// what a row leaves behind: m, log S and the log-probability of its target (MODE_SCORE: that and the row's logsumexp; see put_score for rows that count)
 template <int MODE>
 __device__ __forceinline__ void put_stats(const LossArg& a, int T, long long t, float m, double ls, double lp) {
   if (MODE != MODE_GRAD && a.logp) a.logp[t] = float(lp);
+  if (MODE == MODE_SCORE) a.lse[t] = float(lp);
   if (MODE != MODE_STATS) return;
   if (a.logp64) a.logp64[t] = lp;
   if (a.stats) {
     a.stats[t] = m;
     a.stats[T + t] = float(ls);
   }
+}
+
+__device__ __forceinline__ void put_score(const LossArg& a, long long t, bool in, float m, float s) {
+  score_of(m, double(s), a.zy[t], in, a.logp[t], a.lse[t]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -449,6 +441,10 @@ __global__ void __launch_bounds__(WARP ? WARP_ROWS * 32 : ROW_THREADS, WARP ? 5 
       row_stats<T, 2>(row, r.V, k, m, s, tid, nt);
       join_all(m, s, k);
       const double ls = log64(s), lp64 = double(zy) - double(m) - ls;
+      if (MODE == MODE_SCORE) {
+        if (tid == 0) put_score(a, t, in, m, s);
+        return;
+      }
       float g = 0.f, w = 0.f, l = 0.f, kl = 0.f, clipped = 0.f;
       if constexpr (MODE == MODE_POLICY) {
         w = weight_of(a, t, r.S);
@@ -730,7 +726,7 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
         if (a.old_lp) old_lp = a.old_lp[b.t];
         if (a.ref_lp) ref_lp = a.ref_lp[b.t];
       }
-      if (live && MODE != MODE_STATS) wt = weight_of(a, b.t, r.S);
+      if (live && COUNTED) wt = weight_of(a, b.t, r.S);
 
       for (unsigned left = b.on; left && ok; left &= left - 1, ++n) {
         if (int(n % PIPE_C) != w) continue;
@@ -870,7 +866,14 @@ __global__ void __launch_bounds__(PIPE_WARPS * 32, 1) row_pipe_kernel(const Rows
         } else {
           const float z = __shfl_sync(~0u, zy, l);
           const double lp = double(z) - double(M) - ls;
-          if (rank == 0 && lane == 0) put_stats<MODE>(a, r.T, t, M, ls, lp);
+          if (rank == 0 && lane == 0) {
+            if constexpr (MODE == MODE_SCORE) {
+              const long long y = ld_idx(a.targets, t, a.idx64);
+              put_score(a, t, y >= 0 && y < r.V, M, S);
+            } else {
+              put_stats<MODE>(a, r.T, t, M, ls, lp);
+            }
+          }
           if constexpr (MODE == MODE_POLICY) {
             float loss, kl, clipped, g;
             const double from = a.old_lp ? double(__shfl_sync(~0u, old_lp, l)) : lp;
@@ -1199,7 +1202,8 @@ static void launch_rows_t(const RowsArg& r, const LossArg& a, bool warp, bool pd
 template <int MODE>
 static int launch_rows(const RowsArg& r, const LossArg& a, bool warp, bool behind_small, cudaStream_t st) {
   const bool pdl = pdl_mode() == 2 || (pdl_mode() == 1 && (behind_small || r.T <= PDL_ROWS));
-  if (r.f32) launch_rows_t<float, MODE>(r, a, warp, pdl, st);
+  if constexpr (MODE == MODE_SCORE) launch_rows_t<float, MODE>(r, a, warp, pdl, st);
+  else if (r.f32) launch_rows_t<float, MODE>(r, a, warp, pdl, st);
   else launch_rows_t<__nv_bfloat16, MODE>(r, a, warp, pdl, st);
   return int(cudaGetLastError());
 }
@@ -1280,8 +1284,12 @@ static int launch_pipe(const RowsArg& r, const LossArg& a, const PipeArg& q, cud
   if (r.dz && (((z ^ d) & 15) || (B > 1 && (r.zb - r.db) * es % 16) || (r.S > 1 && (r.zs - r.ds) * es % 16))) return TFB_NOT_TAKEN;
   const bool whole = (z & 15) == 0 && (B == 1 || r.zb * es % 16 == 0) && (r.S == 1 || r.zs * es % 16 == 0);
   const long long bytes = (long long)r.V * es, nvec = whole ? (bytes + 15) / 16 : (bytes + 30) / 16;
-  if (r.dz) return r.f32 ? launch_pipe_t<float, MODE, MODE != MODE_STATS>(r, a, q, nvec, st) : launch_pipe_t<__nv_bfloat16, MODE, MODE != MODE_STATS>(r, a, q, nvec, st);
-  return r.f32 ? launch_pipe_t<float, MODE, false>(r, a, q, nvec, st) : launch_pipe_t<__nv_bfloat16, MODE, false>(r, a, q, nvec, st);
+  if constexpr (MODE == MODE_SCORE) {
+    return launch_pipe_t<float, MODE, false>(r, a, q, nvec, st);
+  } else {
+    if (r.dz) return r.f32 ? launch_pipe_t<float, MODE, MODE != MODE_STATS>(r, a, q, nvec, st) : launch_pipe_t<__nv_bfloat16, MODE, MODE != MODE_STATS>(r, a, q, nvec, st);
+    return r.f32 ? launch_pipe_t<float, MODE, false>(r, a, q, nvec, st) : launch_pipe_t<__nv_bfloat16, MODE, false>(r, a, q, nvec, st);
+  }
 }
 
 // One of the two, and the sums over the rows: out[i], i < nsums.  ws: the workspace of either form (terms or the clusters' sums); *counter is 0.
@@ -1301,12 +1309,13 @@ static int rows_and_sums(const RowsArg& r, LossArg a, int nsums, void* ws, int* 
   return int(cudaGetLastError());
 }
 
-int row_stats(const float* z, long long ldz, int T, int V, const void* targets, int idx64, long long ignore, float* stats, int* status, void* stream) {
+int row_scores(const float* z, long long ldz, int T, int V, const void* targets, int idx64, long long ignore, const float* zy, float* logp, float* lse, int* status,
+               void* stream) {
   RowsArg r = {};
   r.z = z; r.zs = ldz; r.T = r.S = T; r.V = V; r.f32 = 1; r.status = status;
   LossArg a = {};
-  a.targets = targets; a.idx64 = idx64; a.ignore = ignore; a.stats = stats;
-  return rows_and_sums<MODE_STATS>(r, a, 0, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+  a.targets = targets; a.idx64 = idx64; a.ignore = ignore; a.zy = zy; a.logp = logp; a.lse = lse;
+  return rows_and_sums<MODE_SCORE>(r, a, 0, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 static bool bad_rows(const RowsArg& r) { return !r.z || r.T <= 0 || r.S <= 0 || r.V <= 0 || r.T % r.S; }

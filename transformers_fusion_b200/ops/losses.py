@@ -41,7 +41,7 @@ _ROWS = struct.Struct("@PPqqqqiiiiP0P")                      # z, dz, zb, zs, db
 _POLICY = struct.Struct("@PiqPPPiiiifffPPPPPP0P")            # targets, idx64, ignore, adv, old, ref, adv_seq, ratio, kl, mean, lo, hi, kl_coef, n_valid, logp, out, ws, denom, counter
 _PREFERENCE = struct.Struct("@PiqPiiffPPPPPPPP0P")           # targets, idx64, ignore, ref, kind, average, beta, smooth, loss, margins, logp, lp64, stats, coef, terms, counter
 _DISTILL = struct.Struct("@PPiiifPPPPPP0P")                  # ids, z, idx64, top_f32, K, tau, n_valid, kl, loss, ws, denom, counter
-_SCORE = struct.Struct("@PPqqPiqiiiPPPPPqPiPqP0P")           # x, w, ldx, ldw, targets, idx64, ignore, M, V, H, logp, lse, rows, row_of, xc, ldc, part, parts, z, ldz, stats
+_SCORE = struct.Struct("@PPqqPiqiiiPPPPPPqPiPqP0P")          # x, w, ldx, ldw, targets, idx64, ignore, M, V, H, logp, lse, rows, row_of, col_of, xc, ldc, part, parts, z, ldz, zy
 
 _lib.register("tfb_token_logprobs", [c_p, c_p, c_i, c_ll, c_p, c_p, c_p])
 _lib.register("tfb_token_logprobs_bwd", [c_p, c_p, c_i, c_ll, c_p, c_p, c_p])
@@ -510,11 +510,11 @@ def linear_logprobs(x, weight, targets, ignore_index: int = -100):
     parts = 4 * -(-V // (128 if n <= 128 else 256)) * n
     xc, work = _empty(dev, n, H, dtype=torch.bfloat16), _empty(dev, parts + ldz * n + 3 * n + 1)
     ws = work.data_ptr()
-    stats, rows = ws + 4 * (parts + ldz * n), ws + 4 * (parts + ldz * n + 2 * n)
+    zy, rows = ws + 4 * (parts + ldz * n), ws + 4 * (parts + ldz * n + n)
     status = _lib.status_word(dev).data_ptr()
     for a in range(0, M, n):
         arg = _SCORE.pack(x2.data_ptr() + 2 * a * x2.stride(0), w.data_ptr(), x2.stride(0), w.stride(0), y.data_ptr() + y.element_size() * a, y.dtype is torch.int64,
-                          int(ignore_index), min(n, M - a), V, H, lp.data_ptr() + 4 * a, lse.data_ptr() + 4 * a, rows, rows + 4, xc.data_ptr(), H, ws, 0,
-                          ws + 4 * parts if ldz else 0, ldz, stats)
+                          int(ignore_index), min(n, M - a), V, H, lp.data_ptr() + 4 * a, lse.data_ptr() + 4 * a, rows, rows + 4, rows + 4 + 4 * n, xc.data_ptr(), H, ws, 0,
+                          ws + 4 * parts if ldz else 0, ldz, zy)
         _call(dev, "linear_logprobs", 3, _lib.lib().tfb_linear_logprobs, arg, status)
     return lp, lse
