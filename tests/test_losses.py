@@ -720,3 +720,39 @@ def test_scoring_of_nearly_certain_tokens(dev, M, H, V):
     near(got, lp, tol * keep, "logp")
     near(lse, torch.logsumexp(z, 1) * keep, (H * 2 ** -24 * size + REL / 2 + 2 ** -23 * z.abs().max(1).values) * keep, "lse")
     assert (got <= 0).all()
+
+
+def exact_products(M, H, V, g, dev):
+    """States and a head whose products are exact in 32 bits, in any order: multiples of 1/4 up to 1/2, so that sums are multiples of 1/16 below H / 4 < 2^20."""
+    x, w = (torch.randint(-2, 3, (n, H), generator=g, device=g.device).mul(0.25).to(BF).to(dev) for n in (M, V))
+    y = torch.randint(0, V, (M,), generator=g, device=g.device)
+    return x, w, torch.where(torch.rand(M, generator=g, device=g.device) < 0.3, torch.full_like(y, IGN), y).to(dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M,H,V", [(1, 512, 4001), (61, 512, 50257), (64, 64, 33), (65, 256, 1001), (100, 512, 50257), (128, 1024, 777), (128, 64, 129), (100, 2048, 4001), (128, 2048, 513),
+                                   (129, 256, 1001), (400, 512, 9000)])
+def test_scoring_of_exact_products(dev, M, H, V):
+    """What is left is the statistics' own error, a hundredth of one column's part in most of these: every column and row is in its place, in each form of the product."""
+    x, w, y = exact_products(M, H, V, gen("cpu", M + V), dev)
+    keep, lsm = y != IGN, torch.log_softmax(x.double() @ w.double().t(), -1)
+    want = lsm.gather(1, y.clamp(min=0)[:, None])[:, 0] * keep
+    lp, lse = L.linear_logprobs(x, w, y)
+    near(lp, want, lp_tol(want) * keep)
+    want = torch.logsumexp(x.double() @ w.double().t(), -1) * keep
+    near(lse, want, lp_tol(want) * keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("last", [1, 100, 129])
+def test_scoring_of_a_short_last_launch(last):
+    """The rows behind a launch's most take another form of the product, in the workspace of the first."""
+    M, H, V = L.SCORE_ROWS + last, 64, 700
+    x, w, y = exact_products(M, H, V, gen("cuda", last), "cuda")
+    y[-1] = 3
+    keep, z = y != IGN, x.double() @ w.double().t()
+    lp, lse = L.linear_logprobs(x, w, y)
+    want = torch.log_softmax(z, -1).gather(1, y.clamp(min=0)[:, None])[:, 0] * keep
+    near(lp, want, lp_tol(want) * keep)
+    want = torch.logsumexp(z, -1) * keep
+    near(lse, want, lp_tol(want) * keep)
