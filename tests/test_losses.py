@@ -756,3 +756,30 @@ def test_scoring_of_a_short_last_launch(last):
     near(lp, want, lp_tol(want) * keep)
     want = torch.logsumexp(z, -1) * keep
     near(lse, want, lp_tol(want) * keep)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [37, 16400])
+def test_kl_of_the_policys_tokens_and_of_the_references(dev, V):
+    """A uniform policy's tokens are every token once: over them log_ratio and k3 have the mean KL(policy || reference), k1 its negative.  The reference's tokens, when that is the
+    uniform one: k1 has the mean KL(reference || policy).  With a coefficient the gradient is the derivative of that mean."""
+    T = min(V, 400)                                               # a vocabulary whose first T tokens are all that is not masked
+    q = torch.log_softmax(torch.randn(T, generator=gen("cpu", V), dtype=torch.float64), 0)
+    z = torch.full((T, V), -math.inf)
+    z[:, :T] = 0.0
+    y, A, flat = torch.arange(T), torch.zeros(T), torch.full((T,), -math.log(T))
+    z, y, A, other, flat = z.to(dev), y.to(dev), A.to(dev), q.float().to(dev), flat.to(dev)
+    kl_p = (-math.log(T) - q).mean().item()                       # KL(uniform || other) = KL(other || policy) of the second call's roles
+    got = {k: L.policy_loss_fwd_bwd(z, y, A, None, other, clip=None, kl=k, kl_coef=0.5) for k in ("k3", "log_ratio", "k1")}
+    tol = REL * (1 + q.abs().max().item())
+    for k, sign in (("k3", 1), ("log_ratio", 1), ("k1", -1)):
+        assert abs(got[k].kl.item() - sign * kl_p) <= tol and abs(got[k].loss.item() - 0.5 * sign * kl_p) <= tol, k
+    p = torch.softmax(z.double(), -1)
+    hot = torch.zeros_like(p).scatter_(1, y[:, None], 1.0)
+    for k, c in (("log_ratio", 0.5 / T), ("k1", -0.5 / T)):
+        c = torch.full((T,), c, dtype=torch.float64, device=dev)
+        check_grad(got[k].dlogits, z, y, c, F32)
+    zq = z.clone()
+    zq[:, :T] = other
+    o = L.policy_loss_fwd_bwd(zq, y, A, None, flat, clip=None, kl="k1", kl_coef=0.5)
+    assert abs(o.kl.item() - kl_p) <= tol

@@ -27,7 +27,7 @@ struct RowsArg {
 };
 
 enum : int { MODE_STATS = 0, MODE_GRAD = 1, MODE_POLICY = 2, MODE_DISTILL = 3, MODE_SCORE = 4 };
-enum : int { KL_K3 = 0, KL_K1 = 1 };
+enum : int { KL_K3 = 0, KL_K1 = 1, KL_LOG_RATIO = 2 };
 enum : int { MEAN_TOKENS = 0, MEAN_SEQUENCES = 1, MEAN_SUM = 2 };
 
 struct LossArg {
@@ -114,7 +114,7 @@ __device__ __forceinline__ float weight_of(const LossArg& a, long long t, int S)
 // The policy's term of one token: l, its KL estimate, whether the clip took its gradient, and g = dl / dlp.
 //   s = r A, r = exp(lp - old); with a clip the smaller of that and clamp(r) A, whose gradient is 0 where it is the smaller one.
 //   Without older log-probabilities old is lp itself, so that a row without a log-probability (NaN, -inf) has no ratio either: its loss is NaN as its gradient is.
-//   Without a ratio s = A lp.  kl: k3 = exp(x) - 1 - x, k1 = x, x = ref - lp.
+//   Without a ratio s = A lp.  kl: k3 = exp(x) - 1 - x, k1 = x, log_ratio = -x, x = ref - lp.
 __device__ __forceinline__ void policy_terms(const LossArg& a, float lp, float lp_old, float ref_lp, float A, float& l, float& kl, float& clipped, float& g) {
   float s, ds;
   clipped = 0.f;
@@ -131,8 +131,8 @@ __device__ __forceinline__ void policy_terms(const LossArg& a, float lp, float l
   float dkl = 0.f;
   if (a.ref_lp) {
     const float e = expm1f(ref_lp);
-    kl = a.kl_kind == KL_K3 && ref_lp != INFINITY ? e - ref_lp : ref_lp;
-    dkl = a.kl_kind == KL_K3 ? -e : -1.f;
+    kl = a.kl_kind == KL_K3 && ref_lp != INFINITY ? e - ref_lp : a.kl_kind == KL_LOG_RATIO ? -ref_lp : ref_lp;
+    dkl = a.kl_kind == KL_K3 ? -e : a.kl_kind == KL_LOG_RATIO ? 1.f : -1.f;
   }
   // a KL term that is only reported has no part in the loss, not even an infinite one; a NaN has, also where the gradient does not depend on lp
   l = a.kl_coef != 0.f ? fmaf(a.kl_coef, kl, -s) : -s;

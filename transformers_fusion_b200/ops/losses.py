@@ -31,7 +31,7 @@ MAX_TOP = 1024          # entries of a teacher's row
 PIPE_CLUSTERS = 296     # most clusters of one launch, each with three sums of 8 bytes in the workspace
 SCORE_ROWS = 1 << 15    # most rows of one launch of linear_logprobs, whose workspace holds their hidden states and 8 bytes a row per 128 of the vocabulary (512 MB of these)
 
-_KL = {"k3": 0, "k1": 1}
+_KL = {"k3": 0, "k1": 1, "log_ratio": 2}
 _MEAN = {"tokens": 0, "sequences": 1, "sum": 2}
 _KIND = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
@@ -270,7 +270,8 @@ def _policy_statement(logits, targets, advantages, old, ref, lo, hi, ratio, kl_c
     k, dk = torch.zeros_like(lp), torch.zeros_like(lp)
     if ref is not None:
         x = ref.double() - lp
-        k, dk = (torch.where(x == math.inf, x, torch.expm1(x) - x), -torch.expm1(x)) if kl == "k3" else (x, -torch.ones_like(x))
+        k, dk = {"k3": lambda: (torch.where(x == math.inf, x, torch.expm1(x) - x), -torch.expm1(x)), "k1": lambda: (x, -torch.ones_like(x)),
+                 "log_ratio": lambda: (-x, torch.ones_like(x))}[kl]()
     w = keep.double()
     if mean == "tokens":
         w = w / (n_valid.double() if n_valid is not None else w.sum().clamp(min=1))
@@ -290,8 +291,10 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
 
     Per token, with lp its log-probability, A its advantage, r = exp(lp - old): -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef * KL.  ``clip`` is
     one bound for both sides, (lo, hi), or None: no clip.  Without ``old_logprobs`` the tokens are the policy's own: r is 1 and its gradient that
-    of lp; without a clip as well the objective is A lp itself.  KL against ``ref_logprobs``, x = ref - lp: "k3" exp(x) - 1 - x (estimates KL(policy || reference)
-    on the policy's tokens), "k1" x (KL(reference || policy) on the reference's).
+    of lp; without a clip as well the objective is A lp itself.  KL against ``ref_logprobs``, x = ref - lp.  On tokens that the policy sampled, KL(policy || reference) is
+    the mean of "k3" exp(x) - 1 - x and of "log_ratio" -x (lp - ref; often called k1 elsewhere).  On tokens that the reference sampled (an older policy, whose
+    log-probabilities are passed as ``ref_logprobs``), KL(reference || policy) is the mean of "k1" x.  The two have opposite signs: "k1" on the policy's own tokens has a mean
+    of -KL(policy || reference).
 
     ``advantages``: one per token, or [B], one per sequence.  ``mean``: over all "tokens" (``n_valid``, one float32 value above 0 on the device, replaces their
     number, for a batch in several calls), over the "sequences" of each one's mean over its tokens (a sequence without tokens counts as 0), or "sum"."""
