@@ -783,3 +783,20 @@ def test_kl_of_the_policys_tokens_and_of_the_references(dev, V):
     zq[:, :T] = other
     o = L.policy_loss_fwd_bwd(zq, y, A, None, flat, clip=None, kl="k1", kl_coef=0.5)
     assert abs(o.kl.item() - kl_p) <= tol
+
+
+@pytest.mark.gpu
+def test_launches_of_several_kernels_and_cluster_sizes_in_turn():
+    """What is remembered of a launch belongs to its kernel and its size of cluster: calls that alternate between losses, types and vocabularies give what each gives alone."""
+    calls = []
+    for V, dtype in ((9001, BF), (50257, F32), (128256, BF), (140000, F32)):
+        z, y = make("cuda", (40,), V, dtype, V)
+        A, ids = torch.randn(40, generator=gen("cpu", V)).cuda(), torch.randint(0, V, (40, 300), generator=gen("cpu", V)).cuda()
+        top = torch.randn(40, 300, generator=gen("cpu", V)).cuda()
+        calls += [lambda z=z, y=y: L.logprobs_fwd(z, y), lambda z=z, y=y, A=A: L.policy_loss_fwd_bwd(z, y, A)[3:], lambda z=z, ids=ids, top=top: L.distill_loss_fwd_bwd(z, ids, top)[1:],
+                  lambda z=z, y=y, A=A: L.policy_loss_fwd_bwd(z, y, A, want_grad=False)[:1]]
+    alone = [[c() for _ in range(2)][1] for c in calls]
+    for order in (range(len(calls)), reversed(range(len(calls))), list(range(0, len(calls), 3)) * 2):
+        for i in order:
+            assert all(torch.equal(a, b) for a, b in zip(calls[i](), alone[i])), i
+    _lib.check_status()

@@ -1215,16 +1215,21 @@ static bool short_rows(const RowsArg& r, const LossArg& a) {
   return a.K <= WARP_TOP && bytes <= (r.T >= 1024 ? 8192 : 2048);
 }
 
-// Clusters of `kern` that the device holds at a time (0: none; negative: -cudaError_t).  One entry per thread and kernel, since a run repeats its shapes.
-template <class Kern>
-static int resident_clusters(Kern kern, int C, int threads, int smem) {
-  static thread_local int key[4] = {-1, 0, 0, 0}, val = 0;
+// Clusters of C blocks of a kernel that the device holds at a time (0: none; negative: -cudaError_t).  One entry per thread, kernel and size of cluster, since a run repeats its
+// shapes.
+template <class T, int MODE, bool GRAD>
+static int resident_clusters(int C, int smem) {
+  struct Entry { int dev, smem, n; };
+  static thread_local Entry entries[4] = {{-1}, {-1}, {-1}, {-1}};      // C = 1, 2, 4, 8
+  auto kern = row_pipe_kernel<T, MODE, GRAD>;
+  constexpr int threads = PIPE_WARPS * 32;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (key[0] == dev && key[1] == C && key[2] == threads && key[3] == smem) return val;
+  Entry& e = entries[C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3];
+  if (e.dev == dev && e.smem == smem) return e.n;
   int n = 0;
   if (C == 1) {
-    if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem)) return -int(e);
+    if (cudaError_t err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem)) return -int(err);
     n *= sm_count();
   } else {
     cudaLaunchConfig_t cfg = {};
@@ -1232,10 +1237,10 @@ static int resident_clusters(Kern kern, int C, int threads, int smem) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = C; cfg.blockDim = threads; cfg.dynamicSmemBytes = smem; cfg.attrs = at; cfg.numAttrs = 1;
-    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) return -int(e);
+    if (cudaError_t err = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) return -int(err);
   }
-  key[0] = dev; key[1] = C; key[2] = threads; key[3] = smem;
-  return val = n;
+  e = {dev, smem, n};
+  return n;
 }
 
 template <class T, int MODE, bool GRAD>
@@ -1257,7 +1262,7 @@ static int launch_pipe_t(const RowsArg& r, const LossArg& a, PipeArg q, long lon
   q.vs = int((nvec + C - 1) / C);
   const int smem = q.chunks * CHUNK_BYTES + extra;
   if (int e = ensure_dyn_smem(once, kern, most)) return e;
-  const int n = resident_clusters(kern, C, PIPE_WARPS * 32, smem);
+  const int n = resident_clusters<T, MODE, GRAD>(C, smem);
   if (n < 0) return -n;
   if (n == 0) return TFB_NOT_TAKEN;
   q.clusters = min(min(n, PIPE_CLUSTERS), r.T);
