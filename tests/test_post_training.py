@@ -348,3 +348,21 @@ def test_a_run_of_them(dev):
         assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
     else:                       # the embedding's gradient is added up in no fixed order: a weight may round to its neighbour (2^-8)
         assert ((first[0] - second[0]).abs() <= 2e-2 * first[0].abs() + 2e-2).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["dense", "other"])
+def test_harness_without_a_context(dev, kind):
+    """An empty context: the continuation's first token is scored by the last position, the others by the one before them."""
+    m = model(dev)
+    ids = batch(dev)[0][0, :6].tolist()
+    with torch.no_grad():
+        lp = torch.log_softmax(m(torch.tensor([ids], device=dev)).double(), -1)[0]
+        if kind == "other":
+            m = Squashed(m)
+            lp = torch.log_softmax(m(torch.tensor([ids], device=dev)).double(), -1)[0]
+    for ctx in range(4):
+        at = [(ctx - 1 + i) % 6 for i in range(6 - ctx)]
+        want = lp[at, ids[ctx:]].mean().item()
+        # logits of the dense model are bfloat16 on the GPU and rounded nowhere in its scoring: 2^-9 of values below 8
+        assert abs(ED.EvalHarness(m)._seq_logp(ids[:ctx], ids[ctx:]) - want) <= (2 * 8 * 2 ** -9 if dev == "cuda" else 1e-5 * abs(want)), ctx

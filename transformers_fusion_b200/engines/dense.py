@@ -672,7 +672,8 @@ class EvalHarness:
     def _seq_logp(self, ctx: Sequence[int], cont: Sequence[int]) -> float:
         dev = next(self.model.parameters()).device
         ids = torch.tensor([list(ctx) + list(cont)], device=dev)
-        at = slice(len(ctx) - 1, len(ctx) + len(cont) - 1)
+        # every token by the position before it; without a context the first one has none, and is scored by the last position
+        at = torch.arange(len(ctx) - 1, len(ctx) + len(cont) - 1, device=dev) % max(1, ids.shape[1])
         targets = torch.full_like(ids, -100)
         targets[0, at] = ids[0, len(ctx):]
         score = self.model.score_tokens if ends_in_head(self.model) else lambda ids, targets: L.token_logprobs(self.model(ids).float(), targets)
