@@ -366,3 +366,26 @@ def test_harness_without_a_context(dev, kind):
         want = lp[at, ids[ctx:]].mean().item()
         # logits of the dense model are bfloat16 on the GPU and rounded nowhere in its scoring: 2^-9 of values below 8
         assert abs(ED.EvalHarness(m)._seq_logp(ids[:ctx], ids[ctx:]) - want) <= (2 * 8 * 2 ** -9 if dev == "cuda" else 1e-5 * abs(want)), ctx
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("scope", ["model", "global"])
+def test_hooks_on_what_a_model_is_called_with(dev, scope):
+    """A hook in front of the forward pass changes what is scored, and sees every call of a trainer."""
+    m = model(dev)
+    ids = batch(dev)[0][:1, :9]
+    plain = ED.EvalHarness(m)._seq_logp(ids[0, :5].tolist(), ids[0, 5:].tolist())
+    swapped = (ids + 1) % 96
+    swapped[0, 5:] = ids[0, 5:]
+    want = ED.EvalHarness(m)._seq_logp(swapped[0, :5].tolist(), ids[0, 5:].tolist())
+    assert abs(plain - want) > 1e-2
+
+    def hook(mod, args):
+        return (torch.cat([(args[0][:, :5] + 1) % 96, args[0][:, 5:]], 1),) if mod is m else None
+    handle = m.register_forward_pre_hook(hook) if scope == "model" else torch.nn.modules.module.register_module_forward_pre_hook(hook)
+    try:
+        got = ED.EvalHarness(m)._seq_logp(ids[0, :5].tolist(), ids[0, 5:].tolist())
+    finally:
+        handle.remove()
+    assert abs(got - want) <= (2 * 8 * 2 ** -9 if dev == "cuda" else 1e-5 * abs(want))
+    assert ED.EvalHarness(m)._seq_logp(ids[0, :5].tolist(), ids[0, 5:].tolist()) == plain

@@ -572,10 +572,11 @@ class _FinalNormFn(torch.autograd.Function):
 
 
 def ends_in_head(model) -> bool:
-    """Whether ``model(ids)`` is the forward pass of ``DenseModel`` and nothing sees or changes the logits that it returns (another forward pass, hooks): they are
-    the head's product with ``hidden_states`` then, and nobody else's."""
+    """Whether ``model(ids)`` is the forward pass of ``DenseModel`` and nothing sees or changes what it is called with or the logits that it returns (another forward pass,
+    hooks): they are the head's product with ``hidden_states`` then, and nobody else's."""
+    every = torch.nn.modules.module
     return (isinstance(model, DenseModel) and type(model).forward is DenseModel.forward and "forward" not in vars(model)
-            and not model._forward_hooks and not torch.nn.modules.module._global_forward_hooks)
+            and not (model._forward_hooks or model._forward_pre_hooks or every._global_forward_hooks or every._global_forward_pre_hooks))
 
 
 class _LinearFn(torch.autograd.Function):
