@@ -389,3 +389,52 @@ def test_hooks_on_what_a_model_is_called_with(dev, scope):
         handle.remove()
     assert abs(got - want) <= (2 * 8 * 2 ** -9 if dev == "cuda" else 1e-5 * abs(want))
     assert ED.EvalHarness(m)._seq_logp(ids[0, :5].tolist(), ids[0, 5:].tolist()) == plain
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_logits_of_other_layouts(dev):
+    """Logits whose last dimension is not dense, of a type that the losses do not take, and of more rows and positions than there are tokens."""
+    g = torch.Generator().manual_seed(2)
+    z = torch.randn(4, 9, 30, generator=g).to(dev)
+    ids = torch.randint(0, 30, (3, 7), generator=g).to(dev)
+    f = rl.GRPOTrainer.compute_log_probs
+    want = torch.log_softmax(z.double()[:3, :6], -1).gather(-1, ids[:, 1:, None])[..., 0]
+    apart = z.transpose(1, 2).contiguous().transpose(1, 2)
+    assert apart.stride(-1) != 1
+    # 2^-24 of a sum of 30 terms on its way, and half a step of values below 16
+    for t, tol in ((z, 4e-6), (apart, 4e-6), (apart[:3, :7], 4e-6), (z.double(), 4e-6), (apart.half(), 2 ** -11 * 16)):
+        assert (f(t, ids) - want).abs().max() <= tol
+    leaf = apart.clone(memory_format=torch.preserve_format).requires_grad_(True)
+    f(leaf, ids).sum().backward()
+    p = torch.softmax(z.double(), -1)
+    grad = torch.zeros_like(p)
+    grad[:3, :6] = torch.zeros_like(p[:3, :6]).scatter_(-1, ids[:, 1:, None], 1.0) - p[:3, :6]
+    assert leaf.stride() == apart.stride() and (leaf.grad - grad).abs().max() <= 4e-6
+    with pytest.raises(ValueError):
+        f(z[:2], ids)
+
+    class Fixed(torch.nn.Module):
+        def forward(self, ids):
+            return apart[:3, :7]
+    assert (rl.token_logprobs(Fixed(), ids) - want).abs().max() <= 4e-6
+    assert (rl.score_tokens(Fixed(), ids, rl.next_tokens(ids))[:, :-1] - want).abs().max() <= 4e-6
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_policy_grad_loss_of_other_arguments(dev):
+    """Logits whose last dimension is not dense, one advantage for all rows, advantages of other types, labels below 0 that are not the ignored one (they count as 0)."""
+    g = torch.Generator().manual_seed(3)
+    z = torch.randn(7, 10, generator=g).to(dev).t()
+    y = torch.randint(0, 7, (10,), generator=g).to(dev)
+    y[2], y[5] = -100, -1
+    keep = y != -100
+    for adv in (torch.randn(10, generator=g).to(dev), torch.randn(1, generator=g).to(dev), torch.tensor(2.0, device=dev), torch.arange(10, device=dev)):
+        loss, d = ED.policy_grad_loss(z, y, adv)
+        t = z.double().requires_grad_(True)
+        want = -(adv.double() * torch.log_softmax(t, -1).gather(1, y.clamp(min=0)[:, None])[:, 0] * keep).sum() / keep.sum()
+        want.backward()
+        assert loss == pytest.approx(float(want.detach()), rel=1e-5, abs=1e-6) and (d - t.grad).abs().max() < 1e-5 * adv.abs().max().item() + 1e-6
+    ids, top = torch.rand(10, 7, generator=g).argsort(-1)[:, :3].to(dev), torch.randn(10, 3, generator=g).to(dev)
+    assert torch.equal(ED.distill_top_loss(z, ids, top)[1], ED.distill_top_loss(z.contiguous(), ids, top)[1])
+    pairs, labels = torch.randn(2, 7, 5, generator=g).to(dev).transpose(1, 2), y[6:].clamp(min=0).repeat(2, 2)[:, :5]
+    assert torch.equal(ED.preference_loss(pairs, labels)[1], ED.preference_loss(pairs.contiguous(), labels)[1])

@@ -293,6 +293,10 @@ def _rows(logits, labels):
     return logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1)
 
 
+def _dense(lg):
+    return lg if lg.stride(-1) == 1 else lg.contiguous()
+
+
 def _acc(lg, lab, keep):
     return float((lg.argmax(-1)[keep] == lab[keep]).float().mean()) if keep.any() else 0.0
 
@@ -570,23 +574,25 @@ def normalize_rewards(rewards: torch.Tensor) -> RewardStats:
 
 
 def policy_grad_loss(logits, labels, advantages, ignore_index: int = -100):
-    """REINFORCE surrogate -(A * log pi(label)) averaged over kept rows; advantages per row.  Returns (loss, dlogits)."""
+    """REINFORCE surrogate -(A * log pi(label)) averaged over kept rows; advantages per row, or one for all.  Returns (loss, dlogits)."""
     lg, lab = _rows(logits, labels)
-    o = L.policy_loss_fwd_bwd(lg, lab, advantages.float().reshape(-1), clip=None, ignore_index=ignore_index)
+    adv = advantages.float().reshape(-1)
+    o = L.policy_loss_fwd_bwd(_dense(lg), torch.where(lab == ignore_index, lab, lab.clamp(min=0)), adv.expand(lab.shape) if adv.numel() == 1 else adv, clip=None,
+                              ignore_index=ignore_index)
     return float(o.loss), o.dlogits.view(logits.shape)
 
 
 def distill_top_loss(logits, top_ids, top_logits, temperature: float = 1.0):
     """Distillation from a teacher's top logits [..., K]: temperature^2 times the mean KL over the rows with entries (ids of -1: none).  Returns
     (loss, dlogits)."""
-    o = L.distill_loss_fwd_bwd(logits.float().reshape(-1, logits.shape[-1]), top_ids.reshape(-1, top_ids.shape[-1]), top_logits.reshape(-1, top_ids.shape[-1]),
+    o = L.distill_loss_fwd_bwd(_dense(logits.float().reshape(-1, logits.shape[-1])), top_ids.reshape(-1, top_ids.shape[-1]), top_logits.reshape(-1, top_ids.shape[-1]),
                                temperature=temperature)
     return float(o.loss), o.dlogits.view(logits.shape)
 
 
 def preference_loss(logits, labels, ref_logp=None, beta: float = 0.1, label_smoothing: float = 0.0, ignore_index: int = -100):
     """Loss of N pairs (logits [2N, S, V], labels [2N, S]: chosen answers first).  Returns (LossOut with the share of pairs in the right order, dlogits)."""
-    o = L.preference_loss_fwd_bwd(logits.float(), labels, ref_logp, beta=beta, label_smoothing=label_smoothing, ignore_index=ignore_index)
+    o = L.preference_loss_fwd_bwd(_dense(logits.float()), labels, ref_logp, beta=beta, label_smoothing=label_smoothing, ignore_index=ignore_index)
     return LossOut(float(o.loss), float((o.margins > 0).float().mean())), o.dlogits
 
 

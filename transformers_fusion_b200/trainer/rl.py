@@ -46,8 +46,9 @@ def next_tokens(ids, mask=None):
 
 
 def _loss_logits(logits):
-    """Logits of a type that the losses take."""
-    return logits if logits.dtype in (torch.bfloat16, torch.float32) else logits.float()
+    """Logits of a type and layout that the losses take."""
+    logits = logits if logits.dtype in (torch.bfloat16, torch.float32) else logits.float()
+    return logits if logits.stride(-1) == 1 else logits.contiguous()
 
 
 def score_tokens(model, ids, targets):
@@ -59,7 +60,14 @@ def score_tokens(model, ids, targets):
 
 def token_logprobs(model, ids):
     """log p(ids[:, t+1] | ids[:, :t+1]) for t = 0..S-2 -> [B, S-1] (graph attached)."""
-    return L.token_logprobs(_loss_logits(model(ids)), next_tokens(ids))[:, :-1]
+    return _next_logprobs(model(ids), ids)
+
+
+def _next_logprobs(logits, ids):
+    """log p of the tokens that follow, [B, S - 1], of logits of at least ids' rows and positions."""
+    if logits.shape[:2] != ids.shape:
+        logits = logits[:ids.shape[0], :ids.shape[1]]
+    return L.token_logprobs(_loss_logits(logits), next_tokens(ids))[:, :-1]
 
 
 class _RLBase:
@@ -99,7 +107,7 @@ class _RLBase:
     @staticmethod
     def compute_log_probs(logits, ids):
         """log p of the tokens that follow: logits [B, S, V], ids [B, S] -> [B, S-1] (position t scores ids[:, t+1])."""
-        return L.token_logprobs(_loss_logits(logits), next_tokens(ids))[:, :-1]
+        return _next_logprobs(logits, ids)
 
     @staticmethod
     def compute_kl_divergence(logits_a, logits_b) -> float:
