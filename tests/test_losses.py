@@ -800,3 +800,51 @@ def test_launches_of_several_kernels_and_cluster_sizes_in_turn():
         for i in order:
             assert all(torch.equal(a, b) for a, b in zip(calls[i](), alone[i])), i
     _lib.check_status()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [9, 300])
+def test_transformations_of_token_logprobs(dev, V):
+    """Second derivatives, forward mode, batched gradients and the transformations of torch.func, against the same of the formula in float64.  Every value is made of at most two sums of
+    V terms in 32 bits and products of three numbers up to 8: V 2^-24 * 64 holds them."""
+    g = gen("cpu", V)
+    z, y = make("cpu", (2, 3), V, F32, V, ignored=0.0)
+    y[0, 1], y[1, 2] = IGN, V                                     # an ignored row, and a target outside the vocabulary in the last one
+    v, d = torch.randn(2, 3, V, generator=g), torch.randn(5, 2, 3, generator=g)
+    z, y, v, d = z.to(dev), y.to(dev), v.to(dev), d.to(dev)
+    ok = torch.ones(2, 3, dtype=torch.bool, device=dev)
+    ok[1, 2] = False                                              # its results are NaN in all of them
+    f = lambda t: L.token_logprobs(t, y)
+    f64 = lambda t: torch.log_softmax(t, -1).gather(-1, y.clamp(0, V - 1)[..., None])[..., 0] * (y != IGN)
+    z64, tol = z.double(), 64 * V * 2 ** -24
+
+    def same(got, want, rows):
+        at = (..., rows, slice(None)) if want.shape[-1] == V else (..., rows)
+        near(got[at], want[at], tol)
+    a, b = z.clone().requires_grad_(True), z64.clone().requires_grad_(True)
+    (ga,), (gb,) = torch.autograd.grad(f(a), a, d[0], create_graph=True), torch.autograd.grad(f64(b), b, d[0].double(), create_graph=True)
+    same(ga.detach(), gb.detach(), ok)
+    (ha,), (hb,) = torch.autograd.grad((ga * v)[ok].sum(), a), torch.autograd.grad((gb * v)[ok].sum(), b)
+    same(ha, hb, ok)
+    w = torch.ones(2, 3, device=dev, requires_grad=True)          # and of the gradient that is handed in
+    (gw,) = torch.autograd.grad(f(a), a, w, create_graph=True)
+    (dw,) = torch.autograd.grad((gw * v)[ok].sum(), w)
+    w64 = torch.ones(2, 3, device=dev, dtype=torch.float64, requires_grad=True)
+    (dw64,) = torch.autograd.grad((torch.autograd.grad(f64(b), b, w64, create_graph=True)[0] * v)[ok].sum(), w64)
+    same(dw, dw64, ok)
+    many, many64 = torch.autograd.grad(f(a), a, d, is_grads_batched=True)[0], torch.autograd.grad(f64(b), b, d.double(), is_grads_batched=True)[0]
+    same(many, many64, ok)
+    along = torch.func.jvp(f64, (z64,), (v.double(),))[1]
+    same(torch.func.jvp(f, (z,), (v,))[1], along, ok)
+    with torch.autograd.forward_ad.dual_level():
+        same(torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(z, v))).tangent, along, ok)
+    stack = torch.stack([z, z + v])
+    same(torch.func.vmap(f)(stack), torch.stack([f64(t) for t in stack.double()]), ok)
+    same(torch.func.vmap(torch.func.grad(lambda t: (f(t) * d[0])[ok].sum()))(stack),
+         torch.stack([torch.func.grad(lambda t: (f64(t) * d[0])[ok].sum())(t) for t in stack.double()]), ok)
+    rows = torch.func.vmap(L.token_logprobs)(stack.flatten(0, 1), torch.cat([y, y]))      # targets that are mapped over too
+    same(rows.view(2, 2, 3), torch.stack([f64(t) for t in stack.double()]), ok)
+    for got in (f(z), ga.detach()[..., 0], torch.func.vmap(f)(stack)[0]):
+        assert got[~ok].isnan().all()
+    with pytest.raises(ValueError):
+        torch.func.vmap(L.token_logprobs)(stack.flatten(0, 1), torch.cat([y, y])[:, :2])

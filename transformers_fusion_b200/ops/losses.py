@@ -23,6 +23,7 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import c_i, c_ll, c_p, check
@@ -222,6 +223,23 @@ def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=No
     return grad
 
 
+def _statement(logits, targets, ignore_index):
+    """What ``token_logprobs`` computes, in operations that any transformation goes through; and (kept rows, clamped targets, logits that are 0 on the other rows)."""
+    keep, V = targets != ignore_index, logits.shape[-1]
+    z = torch.where(keep[..., None], logits.float(), torch.zeros((), device=logits.device))
+    y = targets.long()
+    inside, y = (y >= 0) & (y < V), y.clamp(0, V - 1)
+    lp = torch.log_softmax(z, -1).gather(-1, y[..., None])[..., 0]
+    lp = torch.where(inside, lp, torch.full((), math.nan, device=logits.device))
+    return torch.where(keep, lp, torch.zeros((), device=logits.device)), (keep, y, z)
+
+
+def _transformed(*tensors):
+    """Whether a tensor belongs to a function transformation (vmap, grad, jvp ...) or carries a tangent: a kernel sees neither."""
+    return (any(torch._C._functorch.is_functorch_wrapped_tensor(t) or torch._C._functorch.is_legacy_batchedtensor(t) for t in tensors)
+            or forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t.is_floating_point()))
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index):
@@ -231,14 +249,25 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dlogp):
         logits, targets, stats = ctx.saved_tensors
+        if torch.is_grad_enabled() or _transformed(dlogp):
+            # a gradient that is differentiated again (create_graph), or one of many at once
+            lp, (keep, y, z) = _statement(logits, targets, ctx.ignore_index)
+            c = torch.where(keep, torch.where(lp.isnan(), lp, dlogp.float()), torch.zeros((), device=logits.device))
+            hot = torch.zeros_like(z).scatter_(-1, y[..., None], 1.0)
+            return (c[..., None] * (hot - torch.softmax(z, -1))).to(logits.dtype), None, None
         return logprobs_bwd(dlogp.float(), logits, targets, stats, ctx.ignore_index), None, None
 
 
 def token_logprobs(logits, targets, ignore_index: int = -100):
-    """Log-probabilities of given tokens, float32 of the targets' shape, with the gradient of the logits."""
+    """Log-probabilities of given tokens, float32 of the targets' shape, with the gradient of the logits.  Second derivatives, forward-mode ones and the
+    transformations of ``torch.func`` go through tensor operations."""
+    if _transformed(logits, targets):
+        _check_logits(logits)
+        if targets.shape != logits.shape[:-1]:
+            raise ValueError(f"targets: {tuple(logits.shape[:-1])} wanted, got {tuple(targets.shape)}")
+        return _statement(logits, targets, ignore_index)[0]
     return _TokenLogprobs.apply(logits, targets, ignore_index)
 
 
