@@ -438,3 +438,99 @@ def test_policy_grad_loss_of_other_arguments(dev):
     assert torch.equal(ED.distill_top_loss(z, ids, top)[1], ED.distill_top_loss(z.contiguous(), ids, top)[1])
     pairs, labels = torch.randn(2, 7, 5, generator=g).to(dev).transpose(1, 2), y[6:].clamp(min=0).repeat(2, 2)[:, :5]
     assert torch.equal(ED.preference_loss(pairs, labels)[1], ED.preference_loss(pairs.contiguous(), labels)[1])
+
+
+def weighted(mask, seed=3):
+    """Tokens that count by a weight: 0 where the mask is 0, else 0.25 to 2, one of them negative."""
+    w = mask * (0.25 + 1.75 * torch.rand(mask.shape, generator=torch.Generator().manual_seed(seed))).to(mask.device)
+    w[0, 5] = -0.5
+    return w
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("clip,kl", [(0.0, 0.0), (0.2, 0.1)])
+@pytest.mark.parametrize("kind", ["weights", "one_row"])
+def test_grpo_mask_of_weights(dev, clip, kl, kind):
+    m = model(dev)
+    t = rl.GRPOTrainer(m, group_size=4, beta=0.04, clip_eps=clip, kl_coef=kl)
+    if kl:
+        t.ref_model = model(dev, seed=7).eval()
+    ids, mask, _ = batch(dev)
+    mask = weighted(mask) if kind == "weights" else mask[1:2]
+    rewards = torch.tensor([1.0, 0.2, -0.5, 0.7])
+    got, loss = stepped_gradients(t, lambda: t.train_step(ids, mask, rewards))
+    adv = t.advantages(rewards).to(dev)[:, None]
+
+    def plain():
+        lp, k = lp64(m, ids), mask[:, 1:]
+        n = k.sum(-1).clamp(min=1)
+        per = -torch.exp(lp - lp.detach()) * adv if clip else -adv * lp
+        out = ((per * k).sum(-1) / n).mean()
+        if kl:
+            with torch.no_grad():
+                r = lp64(t.ref_model, ids)
+            out = out + kl * (((torch.exp(r - lp) - (r - lp) - 1) * k).sum(-1) / n).mean()
+        return out
+    want, wloss = plain_gradients(m, plain)
+    same(got, want * (1 - 0.01 * 0.04), dev)
+    assert loss == pytest.approx(wloss, rel=1e-4, abs=1e-4) and t.last_loss() == loss
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("given", [False, True])
+def test_ppo_mask_of_weights(dev, given):
+    m = model(dev)
+    t = rl.PPOTrainer(m)
+    ids, mask, g = batch(dev)
+    mask = weighted(mask).abs()
+    k = mask[:, 1:]
+    old = None
+    if given:
+        with torch.no_grad():
+            old = (lp64(m, ids) + 0.1 * torch.randn(4, 16, generator=g).to(dev)).masked_fill(k == 0, float("nan"))
+    coef, rewards = t.kl_coef, [1.0, 0.0, -1.0, 0.5]
+    v = t.values(ids).detach()
+    got, (loss, vloss, kl) = stepped_gradients(t, lambda: t.train_step(ids, mask, torch.tensor(rewards), old))
+    advs = []
+    for b, r1 in enumerate(rewards):
+        r = torch.zeros(16)
+        r[int(k[b].nonzero().max())] = r1
+        advs.append(rl.gae(r, torch.cat([v[b, :16].cpu(), torch.zeros(1)]), 0.99, 0.95)[0])
+    adv = torch.stack(advs).to(dev)
+    adv = (adv - (adv * k).sum() / k.sum()) / (adv[k > 0].std() + 1e-8)
+    seen = {}
+
+    def plain():
+        lp = lp64(m, ids)
+        o = lp.detach() if old is None else old.nan_to_num(0.0)
+        r = torch.exp(lp - o)
+        pol = -torch.minimum(r * adv, r.clamp(0.8, 1.2) * adv)
+        seen["kl"] = float((((o - lp) * k).sum() / k.sum()).detach())
+        return (pol * k).sum() / k.sum() + coef * ((o - lp) * k).sum() / k.sum()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-3, abs=1e-3) and kl == pytest.approx(seen["kl"], abs=1e-3)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["weights", "one_row"])
+def test_dpo_mask_of_weights(dev, kind):
+    m, ref = model(dev), model(dev, seed=3)
+    t = rl.DPOTrainer(m, ref, beta=0.3)
+    seen = []
+    t.set_log_callback(lambda *a: seen.append(a))
+    (c, cm, _), (r, rm, _) = batch(dev, S=17), batch(dev, S=12, seed=5)
+    cm, rm = (weighted(cm), weighted(rm, 4)) if kind == "weights" else (cm[1:2], rm)
+    got, (loss, acc) = stepped_gradients(t, lambda: t.train_step(c, r, cm, rm))
+    f = lambda q, i, k: (lp64(q, i) * k[:, 1:]).sum(-1)
+    with torch.no_grad():
+        rc, rr = f(ref, c, cm), f(ref, r, rm)
+        gap = float((f(m, c, cm) - rc).mean())
+        order = float((((f(m, c, cm) - rc) - (f(m, r, rm) - rr)) > 0).float().mean())
+
+    def plain():
+        return -torch.nn.functional.logsigmoid(0.3 * ((f(m, c, cm) - rc) - (f(m, r, rm) - rr))).mean()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-4 if dev == "cpu" else 2e-2) and (acc == order or dev == "cuda")
+    assert seen[0][0] == loss and seen[0][1] == pytest.approx(gap, abs=1e-4 if dev == "cpu" else 14 * 8 * 2 ** -9)      # a product of other rows may round a logit to its neighbour, in 14 tokens at most

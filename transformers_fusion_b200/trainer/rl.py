@@ -45,6 +45,11 @@ def next_tokens(ids, mask=None):
     return out
 
 
+def _weights(mask):
+    """Whether a mask holds other weights than 0 and 1: the fused losses know tokens that count and tokens that do not."""
+    return bool(((mask != 0) & (mask != 1)).any())
+
+
 def _loss_logits(logits):
     """Logits of a type and layout that the losses take."""
     logits = logits if logits.dtype in (torch.bfloat16, torch.float32) else logits.float()
@@ -85,8 +90,21 @@ class _RLBase:
         z = logits.detach()
         return logits, z, z if ends_in_head(self.model) else None
 
+    def _through_logprobs(self, parts, objective, grad_scale=1.0):
+        """One step on an objective of the tokens' log-probabilities in tensor operations, for what the fused losses do not state: parts [(ids, targets)] are a forward
+        pass each, ``objective`` takes their log-probabilities [B, S] (0 where there is no target) and returns the loss.  Returns (loss, log-probabilities)."""
+        passes = [self._forward(ids) for ids, _ in parts]
+        scored = [L.logprobs_fwd(z, targets) for (_, z, _), (_, targets) in zip(passes, parts)]
+        lps = [lp.requires_grad_(True) for lp, _ in scored]
+        with torch.enable_grad():
+            loss = objective(*lps)
+        d = torch.autograd.grad(loss, lps)
+        grads = [L.logprobs_bwd(d[i], z, parts[i][1], scored[i][1], out=out) for i, (_, z, out) in enumerate(passes)]
+        self._backward_and_step([logits for logits, _, _ in passes], grads, grad_scale)
+        return loss.detach(), [lp.detach() for lp in lps]
+
     def _backward_and_step(self, logits, dlogits, grad_scale=1.0):
-        logits.backward(dlogits)
+        torch.autograd.backward(logits, dlogits)
         for p in self.flat.params_list:      # tensors that went through plain autograd
             if p.grad is not None:
                 p.main_grad.add_(p.grad.float())
@@ -156,8 +174,8 @@ class GRPOTrainer(_RLBase):
         return (r - r.mean()) / torch.sqrt(r.var(unbiased=False) + 1e-8)
 
     def train_step(self, ids=None, mask=None, rewards=None, prompt: Optional[List[int]] = None):
-        """Either (ids [G, S], mask [G, S] marking completion tokens, rewards [G]) or ``prompt`` (token ids):
-        the group is then sampled and scored here.  Returns the loss value (0.0 for a no-op step)."""
+        """Either (ids [G, S], mask [G, S] marking completion tokens (or [1, S] for all; other values than 0 and 1 are weights of the tokens), rewards [G]) or ``prompt`` (token
+        ids): the group is then sampled and scored here.  Returns the loss value (0.0 for a no-op step)."""
         dev = self.model.tok_embeddings.device
         if prompt is not None:
             outs = self.generate(prompt, self.G, self.max_new, temperature=1.0)
@@ -174,15 +192,27 @@ class GRPOTrainer(_RLBase):
         self.last_advantages = adv
         if float(rewards.var(unbiased=False)) < 1e-12:
             return 0.0                                    # zero-variance group: no update
+        mask = mask.expand(ids.shape)
         targets = next_tokens(ids, mask)
         ref = score_tokens(self.ref_model, ids, targets) if self.ref_model is not None else None
+        scale = 1.0 - 0.01 * self.beta
+        if _weights(mask):
+            m = mask[:, 1:]
+            mean = lambda v: ((v[:, :-1] * m).sum(-1) / m.sum(-1).clamp(min=1)).mean()
+
+            def objective(lp):
+                a = adv[:, None]
+                r = torch.exp(lp - lp.detach())
+                loss = mean(-torch.minimum(r * a, r.clamp(1 - self.clip_eps, 1 + self.clip_eps) * a) if self.clip_eps > 0 else -a * lp)
+                return loss if ref is None else loss + self.kl_coef * mean(torch.expm1(ref - lp) - (ref - lp))
+            self._last_loss = float(self._through_logprobs([(ids, targets)], objective, scale)[0])
+            return self._last_loss
         logits, z, out = self._forward(ids)
         # the group's tokens are the policy's own: with a clip the ratio is 1, without one the objective is advantage * CE
         o = L.policy_loss_fwd_bwd(z, targets, adv, None, ref, clip=self.clip_eps if self.clip_eps > 0 else None, kl_coef=self.kl_coef if ref is not None else 0.0,
                                   mean="sequences", out=out)
-        self._backward_and_step(logits, o.dlogits, grad_scale=1.0 - 0.01 * self.beta)
-        loss = o.loss
-        self._last_loss = float(loss.detach())
+        self._backward_and_step(logits, o.dlogits, scale)
+        self._last_loss = float(o.loss)
         return self._last_loss
 
 
@@ -241,7 +271,7 @@ class PPOTrainer(_RLBase):
         return self.value_head(h).squeeze(-1)
 
     def train_step(self, ids, mask, rewards, old_logprobs=None):
-        """ids [B,S]; mask marks action tokens; rewards [B] terminal rewards."""
+        """ids [B,S]; mask marks action tokens (other values than 0 and 1 are weights); rewards [B] terminal rewards."""
         dev = self.model.tok_embeddings.device
         ids, mask = ids.to(dev), mask.to(dev).float()
         m = mask[:, 1:]
@@ -260,16 +290,29 @@ class PPOTrainer(_RLBase):
         adv = (adv - (adv * m).sum() / m.sum().clamp(min=1)) / (adv[m > 0].std() + 1e-8 if (m > 0).sum() > 1 else 1.0)
         targets = next_tokens(ids, mask)
         pad = lambda t: TF.pad(t.float(), (0, 1))
-        logits, z, out = self._forward(ids)
-        old = L.logprobs_fwd(z, targets)[0] if old_logprobs is None else pad(old_logprobs.to(dev))
-        o = L.policy_loss_fwd_bwd(z, targets, pad(adv), old, old, clip=self.clip, kl_coef=self.kl_coef, kl="k1", out=out)
-        loss, lp = o.loss, o.logp[:, :-1]
-        self._backward_and_step(logits, o.dlogits)
+        if _weights(m):
+            seen = {}
+
+            def objective(lp):
+                lp = lp[:, :-1]
+                old = lp.detach() if old_logprobs is None else torch.where(m != 0, old_logprobs.to(dev).float(), 0.0)
+                r = torch.exp(lp - old)
+                pol = -torch.minimum(r * adv, r.clamp(1 - self.clip, 1 + self.clip) * adv)
+                seen["kl"] = ((old - lp) * m).sum() / m.sum().clamp(min=1)
+                return (pol * m).sum() / m.sum().clamp(min=1) + self.kl_coef * seen["kl"]
+            loss, (lp,) = self._through_logprobs([(ids, targets)], objective)
+            lp, kl = lp[:, :-1], seen["kl"].detach()
+        else:
+            logits, z, out = self._forward(ids)
+            old = L.logprobs_fwd(z, targets)[0] if old_logprobs is None else pad(old_logprobs.to(dev).expand(m.shape))
+            o = L.policy_loss_fwd_bwd(z, targets, pad(adv), old, old, clip=self.clip, kl_coef=self.kl_coef, kl="k1", out=out)
+            loss, lp, kl = o.loss, o.logp[:, :-1], o.kl
+            self._backward_and_step(logits, o.dlogits)
         vloss = (((self.values(ids)[:, :-1] - ret) ** 2) * m).sum() / m.sum().clamp(min=1)
         self.value_opt.zero_grad()
         (self.value_coef * vloss).backward()
         self.value_opt.step()
-        kl = self._last_kl = float(o.kl)
+        kl = self._last_kl = float(kl)
         if getattr(self, "log_cb", None):
             # policy loss, value loss, mean entropy estimate of the action tokens (-log-prob of the taken actions), KL to the old policy
             ent = float((-lp * m).sum() / m.sum().clamp(min=1))
@@ -295,7 +338,13 @@ class DPOTrainer(_RLBase):
     def last_loss(self) -> float: return self._last_loss
 
     def train_step(self, chosen, rejected, chosen_mask, rejected_mask):
+        """Answers [N, S] with their masks (1 on the answer's tokens; other values than 0 and 1 are weights; [1, S] for all).  Returns (loss, share of pairs in the right
+        order)."""
         dev = self.model.tok_embeddings.device
+        chosen, rejected = chosen.to(dev), rejected.to(dev)
+        chosen_mask, rejected_mask = chosen_mask.to(dev).expand(chosen.shape), rejected_mask.to(dev).expand(rejected.shape)
+        if _weights(chosen_mask) or _weights(rejected_mask):
+            return self._step_on_answers([chosen, rejected], [chosen_mask, rejected_mask])
 
         # one batch: the chosen answers, then the rejected ones, padded to one length
         S = max(chosen.shape[1], rejected.shape[1])
@@ -312,6 +361,22 @@ class DPOTrainer(_RLBase):
             # loss and the sequence-level KL estimate to the frozen reference on the chosen answers
             self.log_cb(self._last_loss, float((o.logp[:n] - ref[:n]).mean()))
         return self._last_loss, float((o.margins > 0).float().mean())
+
+    def _step_on_answers(self, ids, masks):
+        """The same with a forward pass to either side, from the tokens' log-probabilities."""
+        targets = [next_tokens(i, m) for i, m in zip(ids, masks)]
+        total = lambda lp, mask: (lp[:, :-1].double() * mask[:, 1:]).sum(-1)      # of an answer: a margin is the difference of long sums
+        ref = [total(score_tokens(self.ref, i, t), m) for i, t, m in zip(ids, targets, masks)]
+        seen = {}
+
+        def objective(*lps):
+            over = [total(lp, m) - r for lp, m, r in zip(lps, masks, ref)]
+            seen["over"], seen["margin"] = over[0].detach(), self.beta * (over[0] - over[1])
+            return -TF.logsigmoid(seen["margin"]).mean()
+        self._last_loss = float(self._through_logprobs(list(zip(ids, targets)), objective)[0])
+        if getattr(self, "log_cb", None):
+            self.log_cb(self._last_loss, float(seen["over"].mean()))
+        return self._last_loss, float((seen["margin"] > 0).float().mean())
 
 
 # ------------------------------------------------------------------------------------------------
