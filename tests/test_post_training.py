@@ -534,3 +534,30 @@ def test_dpo_mask_of_weights(dev, kind):
     same(got, want, dev)
     assert loss == pytest.approx(wloss, rel=1e-4 if dev == "cpu" else 2e-2) and (acc == order or dev == "cuda")
     assert seen[0][0] == loss and seen[0][1] == pytest.approx(gap, abs=1e-4 if dev == "cpu" else 14 * 8 * 2 ** -9)      # a product of other rows may round a logit to its neighbour, in 14 tokens at most
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_ppo_on_its_own_tokens(dev):
+    """Without older log-probabilities the ratio is 1 to the last bit: no token is outside of a clip of width 0, and the KL estimate is 0, which leaves its coefficient alone when
+    that is the target."""
+    m = model(dev)
+    t = rl.PPOTrainer(m, clip=0.0, kl_target=0.0, kl_coef=0.1)
+    ids, mask, _ = batch(dev)
+    v, k = t.values(ids).detach(), mask[:, 1:]
+    rewards = [1.0, 0.0, -1.0, 0.5]
+    got, (loss, _, kl) = stepped_gradients(t, lambda: t.train_step(ids, mask, torch.tensor(rewards)))
+    assert kl == 0.0 and t.kl_coef == 0.1 and t.last_kl() == 0.0
+    advs = []
+    for b, r1 in enumerate(rewards):
+        r = torch.zeros(16)
+        r[int(k[b].nonzero().max())] = r1
+        advs.append(rl.gae(r, torch.cat([v[b, :16].cpu(), torch.zeros(1)]), 0.99, 0.95)[0])
+    adv = torch.stack(advs).to(dev)
+    adv = (adv - (adv * k).sum() / k.sum()) / (adv[k > 0].std() + 1e-8)
+
+    def plain():
+        lp = lp64(m, ids)
+        return -(torch.exp(lp - lp.detach()) * adv * k).sum() / k.sum() + 0.1 * ((lp.detach() - lp) * k).sum() / k.sum()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-4, abs=1e-5)

@@ -290,7 +290,8 @@ class PPOTrainer(_RLBase):
         adv = (adv - (adv * m).sum() / m.sum().clamp(min=1)) / (adv[m > 0].std() + 1e-8 if (m > 0).sum() > 1 else 1.0)
         targets = next_tokens(ids, mask)
         pad = lambda t: TF.pad(t.float(), (0, 1))
-        if _weights(m):
+        if old_logprobs is None or _weights(m):
+            # (the tokens' own log-probabilities as the older ones: from one pass, so that the ratio is 1 and the KL estimate 0 to the last bit)
             seen = {}
 
             def objective(lp):
@@ -304,7 +305,7 @@ class PPOTrainer(_RLBase):
             lp, kl = lp[:, :-1], seen["kl"].detach()
         else:
             logits, z, out = self._forward(ids)
-            old = L.logprobs_fwd(z, targets)[0] if old_logprobs is None else pad(old_logprobs.to(dev).expand(m.shape))
+            old = pad(old_logprobs.to(dev).expand(m.shape))
             o = L.policy_loss_fwd_bwd(z, targets, pad(adv), old, old, clip=self.clip, kl_coef=self.kl_coef, kl="k1", out=out)
             loss, lp, kl = o.loss, o.logp[:, :-1], o.kl
             self._backward_and_step(logits, o.dlogits)
