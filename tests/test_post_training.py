@@ -561,3 +561,34 @@ def test_ppo_on_its_own_tokens(dev):
     want, wloss = plain_gradients(m, plain)
     same(got, want, dev)
     assert loss == pytest.approx(wloss, rel=1e-4, abs=1e-5)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("n,beta", [((1, 3), 0.3), ((4, 1), 0.3), ((4, 4), 0.0), ((4, 4), -0.2)])
+def test_dpo_of_one_answer_against_several(dev, n, beta):
+    """One answer on a side makes a pair with each of the other side's, and a beta that is not above 0 is taken as it is."""
+    m, ref = model(dev), model(dev, seed=3)
+    t = rl.DPOTrainer(m, ref, beta=beta)
+    (c, cm, _), (r, rm, _) = batch(dev, n=n[0], S=17), batch(dev, n=n[1], S=12, seed=5)
+    got, (loss, acc) = stepped_gradients(t, lambda: t.train_step(c, r, cm, rm))
+    f = lambda q, i, k: (lp64(q, i) * k[:, 1:]).sum(-1)
+
+    def plain():
+        with torch.no_grad():
+            rc, rr = f(ref, c, cm), f(ref, r, rm)
+        return -torch.nn.functional.logsigmoid(beta * ((f(m, c, cm) - rc) - (f(m, r, rm) - rr))).mean()
+    want, wloss = plain_gradients(m, plain)
+    if beta:
+        same(got, want, dev)
+    else:
+        assert not got.any() and not want.any()
+    assert loss == pytest.approx(wloss, rel=1e-4 if dev == "cpu" else 2e-2)
+
+
+def test_dpo_of_answers_that_do_not_pair():
+    t = rl.DPOTrainer(model("cpu"))
+    (c, cm, _), (r, rm, _) = batch("cpu", n=2), batch("cpu", n=4)
+    before = t.flat.params.clone()
+    with pytest.raises(ValueError):
+        t.train_step(c, r, cm, rm)
+    assert torch.equal(t.flat.params, before) and t.steps == 0

@@ -339,12 +339,14 @@ class DPOTrainer(_RLBase):
     def last_loss(self) -> float: return self._last_loss
 
     def train_step(self, chosen, rejected, chosen_mask, rejected_mask):
-        """Answers [N, S] with their masks (1 on the answer's tokens; other values than 0 and 1 are weights; [1, S] for all).  Returns (loss, share of pairs in the right
-        order)."""
+        """Answers [N, S] with their masks (1 on the answer's tokens; other values than 0 and 1 are weights; [1, S] for all); one answer on a side is paired with all of the
+        other side's.  Returns (loss, share of pairs in the right order)."""
         dev = self.model.tok_embeddings.device
         chosen, rejected = chosen.to(dev), rejected.to(dev)
+        if len(chosen) != len(rejected) and 1 not in (len(chosen), len(rejected)):
+            raise ValueError(f"as many chosen as rejected answers, or one on a side: got {len(chosen)} and {len(rejected)}")
         chosen_mask, rejected_mask = chosen_mask.to(dev).expand(chosen.shape), rejected_mask.to(dev).expand(rejected.shape)
-        if _weights(chosen_mask) or _weights(rejected_mask):
+        if len(chosen) != len(rejected) or not 0 < self.beta < math.inf or _weights(chosen_mask) or _weights(rejected_mask):
             return self._step_on_answers([chosen, rejected], [chosen_mask, rejected_mask])
 
         # one batch: the chosen answers, then the rejected ones, padded to one length
