@@ -11,6 +11,7 @@ import torch
 from transformers_fusion_b200.engines import dense as ED
 from transformers_fusion_b200.models.config import TransformerConfig
 from transformers_fusion_b200.models.dense import DenseModel
+from transformers_fusion_b200.models.moe import MoEAllConfig, create_moe_variant
 from transformers_fusion_b200.ops import functional as F
 from transformers_fusion_b200.ops import losses as L
 from transformers_fusion_b200.trainer import rl
@@ -592,3 +593,28 @@ def test_dpo_of_answers_that_do_not_pair():
     with pytest.raises(ValueError):
         t.train_step(c, r, cm, rm)
     assert torch.equal(t.flat.params, before) and t.steps == 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("variant,policy", [("EXPERT_CHOICE", "none"), ("SPARSE_TOPK", "token_drop")])
+def test_dpo_of_a_mixture_whose_tokens_compete(dev, variant, policy):
+    """A chosen answer's logits depend neither on the rejected answer nor on padding to its length."""
+    base = TransformerConfig(vocab_size=96, hidden_size=128, num_layers=2, num_heads=2, ffn_hidden_size=192, max_seq_len=64, init_std=0.1)
+    mixture = lambda seed: create_moe_variant(variant, base, MoEAllConfig(num_experts=4, top_k=2, expert_hidden=64, capacity_factor=0.75, capacity_policy=policy), device=dev,
+                                              dtype=torch.float32 if dev == "cpu" else torch.bfloat16, seed=seed)
+    m, ref = mixture(0), mixture(3)
+    t = rl.DPOTrainer(m, ref, beta=0.3)
+    (c, cm, _), (r, rm, _) = batch(dev, S=17), batch(dev, S=12, seed=5)
+    with torch.no_grad():
+        both = m(torch.cat([c, torch.nn.functional.pad(r, (0, 5))]))[:4]
+        assert (both - m(c)).abs().max() > 0.02                       # they do compete
+    got, (loss, acc) = stepped_gradients(t, lambda: t.train_step(c, r, cm, rm))
+
+    def plain():
+        f = lambda q, i, k: (lp64(q, i) * k[:, 1:]).sum(-1)
+        with torch.no_grad():
+            rc, rr = f(ref, c, cm), f(ref, r, rm)
+        return -torch.nn.functional.logsigmoid(0.3 * ((f(m, c, cm) - rc) - (f(m, r, rm) - rr))).mean()
+    want, wloss = plain_gradients(m, plain)
+    same(got, want, dev)
+    assert loss == pytest.approx(wloss, rel=1e-4 if dev == "cpu" else 2e-2)

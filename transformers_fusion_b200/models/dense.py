@@ -579,6 +579,12 @@ def ends_in_head(model) -> bool:
             and not (model._forward_hooks or model._forward_pre_hooks or every._global_forward_hooks or every._global_forward_pre_hooks))
 
 
+def sequences_apart(model) -> bool:
+    """Whether a sequence's logits depend on nothing else in its batch: a decoder of dense blocks.  (The tokens of a batch compete for experts in some mixtures, and what
+    another forward pass does is its own.)"""
+    return ends_in_head(model) and type(model).hidden_states is DenseModel.hidden_states and all(type(blk) is DenseBlock for blk in model.layers)
+
+
 class _LinearFn(torch.autograd.Function):
     """y = x W^T with the weight gradient accumulated into W.main_grad."""
 

@@ -25,7 +25,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 import torch.nn.functional as TF
 
-from ..models.dense import ends_in_head
+from ..models.dense import ends_in_head, sequences_apart
 from ..ops import losses as L
 from .fused_optim import FlatAdamW
 
@@ -346,7 +346,8 @@ class DPOTrainer(_RLBase):
         if len(chosen) != len(rejected) and 1 not in (len(chosen), len(rejected)):
             raise ValueError(f"as many chosen as rejected answers, or one on a side: got {len(chosen)} and {len(rejected)}")
         chosen_mask, rejected_mask = chosen_mask.to(dev).expand(chosen.shape), rejected_mask.to(dev).expand(rejected.shape)
-        if len(chosen) != len(rejected) or not 0 < self.beta < math.inf or _weights(chosen_mask) or _weights(rejected_mask):
+        together = len(chosen) == len(rejected) and sequences_apart(self.model) and sequences_apart(self.ref)
+        if not together or not 0 < self.beta < math.inf or _weights(chosen_mask) or _weights(rejected_mask):
             return self._step_on_answers([chosen, rejected], [chosen_mask, rejected_mask])
 
         # one batch: the chosen answers, then the rejected ones, padded to one length
