@@ -848,3 +848,29 @@ def test_transformations_of_token_logprobs(dev, V):
         assert got[~ok].isnan().all()
     with pytest.raises(ValueError):
         torch.func.vmap(L.token_logprobs)(stack.flatten(0, 1), torch.cat([y, y])[:, :2])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("call", ["logprobs", "policy", "preference", "distill"])
+@pytest.mark.parametrize("other", [False, True], ids=["logits", "tensor"])
+def test_a_graph_that_needs_what_is_written_over(dev, call, other):
+    """A tensor that takes the gradient counts as changed: a graph that has saved it raises in its backward pass, whatever the device."""
+    hidden = torch.randn(2, 3, 8, device=dev, requires_grad=True)
+    logits = hidden @ torch.randn(8, 40, device=dev)
+    buffer = hidden.new_zeros(2, 3, 40)
+    saved = buffer if other else logits
+    loss = (logits * saved).sum() if other else (saved * saved).sum()
+    lp = L.token_logprobs(logits, torch.zeros(2, 3, dtype=torch.int64, device=dev))
+    z, y = logits.detach(), torch.ones(2, 3, dtype=torch.int64, device=dev)
+    ids, c, out = torch.zeros(2, 3, 2, dtype=torch.int64, device=dev), torch.ones(2, 3, device=dev), buffer if other else z
+    before = saved._version
+    {"logprobs": lambda: L.logprobs_bwd(c, z, y, L.logprobs_fwd(z, y)[1], out=out), "policy": lambda: L.policy_loss_fwd_bwd(z, y, c, out=out),
+     "preference": lambda: L.preference_loss_fwd_bwd(z, y, out=out), "distill": lambda: L.distill_loss_fwd_bwd(z, ids, torch.zeros(2, 3, 2, device=dev), out=out)}[call]()
+    assert saved._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    if other:
+        lp.sum().backward()                                       # the logits are as they were
+    else:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            lp.sum().backward()

@@ -24,6 +24,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import c_i, c_ll, c_p, check
@@ -142,8 +143,11 @@ def _rows(logits, grad=None):
     return _ROWS.pack(logits.data_ptr(), dz, st[0], st[1], d[0], d[1], sh[0] * sh[1], max(sh[1], 1), sh[2], f32, status)
 
 
-def _call(device, what, launches, fn, *args):
-    """fn(*args, stream) with the tensors' device current: streams and kernels belong to the device that is."""
+def _call(device, what, launches, fn, *args, out=None):
+    """fn(*args, stream) with the tensors' device current: streams and kernels belong to the device that is.  ``out``: a caller's tensor that is written, of which autograd
+    has to know (a graph that still needs its values raises in its backward pass)."""
+    if out is not None:
+        increment_version(out)
     index = device.index
     if index == torch.cuda.current_device():
         check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what, launches)
@@ -219,7 +223,7 @@ def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=No
         return grad
     if targets.numel():
         _call(logits.device, "token_logprobs_bwd", 1, _lib.lib().tfb_token_logprobs_bwd, _rows(logits, grad), targets.data_ptr(), targets.dtype is torch.int64,
-              int(ignore_index), stats.data_ptr(), dlogp.data_ptr())
+              int(ignore_index), stats.data_ptr(), dlogp.data_ptr(), out=out)
     return grad
 
 
@@ -357,7 +361,7 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     ws = work.data_ptr()
     arg = _POLICY.pack(targets.data_ptr(), targets.dtype is torch.int64, int(ignore_index), advantages.data_ptr(), _at(old), _at(ref), adv_seq, ratio, kl_kind, mean_kind,
                        1 - lo, 1 + hi, float(kl_coef), _at(n_valid), lp.data_ptr(), sums.data_ptr(), ws, ws + 4 * n_ws, ws + 4 * (n_ws + B))
-    _call(dev, "policy_loss", 2, _lib.lib().tfb_policy_loss, _rows(logits, grad), arg)
+    _call(dev, "policy_loss", 2, _lib.lib().tfb_policy_loss, _rows(logits, grad), arg, out=out)
     return PolicyLoss(*sums.unbind(), lp, grad)
 
 
@@ -429,7 +433,7 @@ def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float =
     ws = work.data_ptr()
     arg = _PREFERENCE.pack(targets.data_ptr(), targets.dtype is torch.int64, int(ignore_index), _at(ref), loss_kind, bool(average), float(beta), float(label_smoothing),
                            loss.data_ptr(), margins.data_ptr(), L.data_ptr(), lp64.data_ptr(), ws, ws + 8 * T, ws + 8 * T + 8 * N, ws + 8 * T + 12 * N)
-    _call(dev, "preference_loss", 3 if want_grad else 2, _lib.lib().tfb_preference_loss, _rows(logits, grad), arg)
+    _call(dev, "preference_loss", 3 if want_grad else 2, _lib.lib().tfb_preference_loss, _rows(logits, grad), arg, out=out)
     return PreferenceLoss(loss, margins, L, grad)
 
 
@@ -498,7 +502,7 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     ws = work.data_ptr()
     arg = _DISTILL.pack(top_ids.data_ptr(), top_logits.data_ptr(), top_ids.dtype is torch.int64, top_logits.dtype is torch.float32, K, float(temperature), _at(n_valid),
                         kl.data_ptr(), loss.data_ptr(), ws, ws + 4 * n_ws, ws + 4 * n_ws + 4)
-    _call(dev, "distill_loss", 2, _lib.lib().tfb_distill_loss, _rows(logits, grad), arg)
+    _call(dev, "distill_loss", 2, _lib.lib().tfb_distill_loss, _rows(logits, grad), arg, out=out)
     return DistillLoss(loss, kl, grad)
 
 
