@@ -874,3 +874,35 @@ def test_a_graph_that_needs_what_is_written_over(dev, call, other):
     else:
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             lp.sum().backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_out_that_is_another_input(dev):
+    """A gradient is not written over what its own call still reads: the teacher's logits, the tokens' numbers, the statistics."""
+    V = 6
+    buf = torch.randn(3, 2, V, generator=gen("cpu", 1)).to(dev)
+    z, top = buf[:2], buf[1:]                                     # the teacher's rows are the student's, one further
+    y, ids = torch.zeros(2, 2, dtype=torch.int64, device=dev), torch.arange(V, device=dev).expand(2, 2, V)
+    c = torch.ones(2, 2, device=dev)
+    _, stats = L.logprobs_fwd(z, y)
+    space = torch.zeros(2 * 2 * V + 4, device=dev)
+    out, tail = space[:2 * 2 * V].view(2, 2, V), space[2 * 2 * V - 2:][:4].view(2, 2)
+    apart, whole = space[4:].view(2, 2, V), space[:4].view(2, 2)
+    n = space[3:4]
+    bad = [lambda: L.distill_loss_fwd_bwd(z, ids, top, out=z), lambda: L.distill_loss_fwd_bwd(z, ids, top, n_valid=n, out=out),
+           lambda: L.policy_loss_fwd_bwd(z, y, tail, out=out), lambda: L.policy_loss_fwd_bwd(z, y, c, tail, out=out), lambda: L.policy_loss_fwd_bwd(z, y, c, None, tail, out=out),
+           lambda: L.policy_loss_fwd_bwd(z, y, c, n_valid=n, out=out), lambda: L.preference_loss_fwd_bwd(z, y, tail[0], out=out),
+           lambda: L.logprobs_bwd(tail, z, y, stats, out=out), lambda: L.logprobs_bwd(c, z, y, space[20:].view(2, 2, 2), out=out),
+           lambda: L.logprobs_bwd(c, z, space.view(torch.int64)[:4].view(2, 2), stats, out=out)]
+    before = (buf.clone(), space.clone())
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError(f"call {i} was taken")
+    assert torch.equal(buf, before[0]) and torch.equal(space, before[1])
+    own = L.distill_loss_fwd_bwd(z, ids, z)                       # a teacher that is the student
+    copy = z.clone()
+    assert torch.equal(L.distill_loss_fwd_bwd(copy, ids, copy, out=copy).dlogits, own.dlogits) and own.loss.abs() < 1e-6
+    want = L.policy_loss_fwd_bwd(z, y, c).dlogits                 # next to each other is apart
+    whole.fill_(1.0)
+    assert torch.equal(L.policy_loss_fwd_bwd(z, y, whole, out=apart).dlogits, want) and torch.equal(whole, c)

@@ -13,7 +13,8 @@ tensors run the plain PyTorch statement of the same mathematics.
 Logits are [T, V] or [B, S, V], bfloat16 or float32, of any strides with a dense last dimension (rows may start at any element).  Targets are
 int64 or int32 of the logits' leading shape; rows whose target is ``ignore_index`` are not read, their statistics and gradients are 0.  A
 target outside the vocabulary makes its row's results NaN.  ``out`` takes the gradient: another tensor of the logits' shape and type, or the
-logits themselves, which are then overwritten; None makes a new one.  Per-row results and losses are float32.
+logits themselves, which are then overwritten; None makes a new one.  It shares no memory with the other inputs (but for teacher's
+logits that are the student's, row for row).  Per-row results and losses are float32.
 
 Reference counterparts: log-probabilities, ratio clipping and KL terms of the RL trainers (src/trainer/trainer_rl.cpp:557-1350)."""
 from __future__ import annotations
@@ -98,14 +99,22 @@ def _one_of(value, choices, name):
     return choices[value]
 
 
-def _gradient(logits, out, want_grad):
-    """Where the gradient goes: None, ``out``, or a new tensor."""
+def _gradient(logits, out, want_grad, *inputs):
+    """Where the gradient goes: None, ``out``, or a new tensor.  ``inputs``: what else the call reads (None: not given)."""
     if not want_grad:
         if out is not None:
             raise ValueError("out: without want_grad there is no gradient")
         return None
     if out is None:
         return torch.empty_like(logits)          # rows of the same alignment as those of the logits where they are dense
+    if out.device == logits.device and out.numel():
+        a, b = _span(out)
+        for t in inputs:
+            if t is not None and t.numel():
+                first, last = _span(t)
+                # (a teacher's logits that are the student's, entry by entry, are read before their row is written)
+                if first < b and a < last and not (first == a and t.shape == out.shape and t.stride() == out.stride()):
+                    raise ValueError("out: overlaps an input that is not the logits")
     if out is logits and logits.is_contiguous():
         return out
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -215,7 +224,7 @@ def logprobs_bwd(dlogp, logits, targets, stats, ignore_index: int = -100, out=No
     targets = _check_index(targets, logits.shape[:-1], "targets", logits.device)
     dlogp = _check_f32(dlogp, targets.shape, "dlogp", logits.device)
     stats = _check_f32(stats, torch.Size((2, *targets.shape)), "stats", logits.device)
-    grad = _gradient(logits, out, True)
+    grad = _gradient(logits, out, True, targets, dlogp, stats)
     if not logits.is_cuda:
         keep, y, lp, soft = _taken(logits.detach(), targets, ignore_index)
         c = torch.where(lp.isnan(), lp, dlogp.detach().double())
@@ -347,7 +356,7 @@ def policy_loss_fwd_bwd(logits, targets, advantages, old_logprobs=None, ref_logp
     if not (lo >= 0 and hi >= 0):
         raise ValueError(f"clip: bounds of 0 or more, got {clip!r}")
     ratio = old is not None or clip is not None
-    grad = _gradient(logits, out, want_grad)
+    grad = _gradient(logits, out, want_grad, targets, advantages, old, ref, n_valid)
     B, S = targets.shape if targets.dim() == 2 else (1, targets.shape[0])
     if not logits.is_cuda:
         return _policy_statement(logits, targets, advantages, old, ref, lo, hi, ratio, kl_coef, kl, mean, n_valid, ignore_index, grad)
@@ -417,7 +426,7 @@ def preference_loss_fwd_bwd(logits, targets, ref_logprobs=None, *, beta: float =
         raise ValueError(f"label_smoothing: in [0, 0.5), of the sigmoid loss, got {label_smoothing} ({kind})")
     N, S = logits.shape[0] // 2, logits.shape[1]
     ref = _check_f32(ref_logprobs, torch.Size((2 * N,)), "ref_logprobs", dev)
-    grad = _gradient(logits, out, want_grad)
+    grad = _gradient(logits, out, want_grad, targets, ref)
     if not logits.is_cuda:
         return _preference_statement(logits, targets, ref, beta, kind, label_smoothing, average, ignore_index, grad)
     margins, L = _empty(dev, N), _empty(dev, 2 * N)
@@ -489,7 +498,7 @@ def distill_loss_fwd_bwd(logits, top_ids, top_logits, *, temperature: float = 1.
     if not 0 < temperature < math.inf:
         raise ValueError(f"temperature: more than 0, got {temperature}")
     n_valid = _check_n_valid(n_valid, dev)
-    grad = _gradient(logits, out, want_grad)
+    grad = _gradient(logits, out, want_grad, top_ids, top_logits, n_valid)
     rows = logits.shape[:-1]
     if not logits.is_cuda:
         return _distill_statement(logits, top_ids, top_logits, temperature, n_valid, grad)
