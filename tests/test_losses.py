@@ -802,6 +802,7 @@ def test_launches_of_several_kernels_and_cluster_sizes_in_turn():
     _lib.check_status()
 
 
+@pytest.mark.filterwarnings("ignore")      # operations that torch maps over one by one
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("V", [9, 300])
 def test_transformations_of_token_logprobs(dev, V):
@@ -906,3 +907,44 @@ def test_out_that_is_another_input(dev):
     want = L.policy_loss_fwd_bwd(z, y, c).dlogits                 # next to each other is apart
     whole.fill_(1.0)
     assert torch.equal(L.policy_loss_fwd_bwd(z, y, whole, out=apart).dlogits, want) and torch.equal(whole, c)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M,H,V", [(200, 64, 1), (70, 64, 2), (3, 64, 300001), (140, 8, 300001)])
+def test_scoring_of_one_column_and_of_many(dev, M, H, V):
+    """A vocabulary of one token, whose log-probability is 0 and whose row has no other columns, and one that no cluster's shared memory holds."""
+    x, w, y = exact_products(M, H, V, gen("cpu", M), dev)
+    y[0] = V - 1
+    keep, z = y != IGN, x.double() @ w.double().t()
+    lp, lse = L.linear_logprobs(x, w, y)
+    want = torch.log_softmax(z, -1).gather(1, y.clamp(min=0)[:, None])[:, 0] * keep
+    near(lp, want, lp_tol(want) * keep)
+    want = torch.logsumexp(z, -1) * keep
+    near(lse, want, lp_tol(want) * keep)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M", [3, 90, 200])
+def test_scoring_of_infinite_logits(dev, M):
+    """Rows: 0 a target whose logit is +inf, 1 another column at +inf, 2 a target at -inf, 3 ordinary, 4 all but the target at -inf."""
+    H, V = 8, 40
+    x, w = torch.zeros(max(M, 5), H), torch.zeros(V, H)
+    w[:, 0] = torch.linspace(-1, 1, V)
+    x[:, 0] = 2.0
+    # a logit is infinite where a state of 3e38 meets a weight of 3e38, with the sign of the weight; the other states are 0 there
+    big = 3e38
+    x[0, 1] = x[1, 2] = x[2, 3] = x[4, 4] = big
+    y = torch.full((max(M, 5),), 7)
+    w[7, 1], w[9, 2], w[7, 3] = big, big, -big
+    w[:, 4], w[7, 4] = -big, 0.0
+    x, w, y = x.to(BF).to(dev)[:M], w.to(BF).to(dev), y.to(dev)[:M]
+    lp, lse = L.linear_logprobs(x, w, y)
+    z = x[:, :1].double() @ w[:, :1].double().t()
+    lsm, other = torch.log_softmax(z, -1)[:, 7], torch.logsumexp(torch.cat([z[:, :7], z[:, 8:]], 1), 1)
+    tol = REL + 2 ** -22
+    want = [(math.nan, math.nan), (math.nan, math.nan), (-math.inf, other[2].item()), None, (0.0, None)]
+    for r in range(M):
+        l, s = want[r] if r < 5 and want[r] else (lsm[r].item(), torch.logsumexp(z[r], 0).item())
+        s = z[r, 7].item() if s is None else s
+        near(lp[r].cpu(), torch.tensor(l), tol, ("logp", r))
+        near(lse[r].cpu(), torch.tensor(s), tol, ("lse", r))
