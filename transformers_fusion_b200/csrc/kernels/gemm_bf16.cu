@@ -1429,7 +1429,7 @@ TFB_API int tfb_gemm_glu(const void* A, long long lda, const void* B, long long 
 // number of parts of a row (`part` holds that many x M entries, at most 2 ceil(N / 128)), or an error.
 // Up to one tile of rows (128) one half of a pair would have nothing to compute: single CTAs, with tiles of 128 columns.  us, the whole of linear_logprobs: 128 x 32000 x
 // 512 21, 128 x 128256 x 512 45.  More rows take pairs of SMs with tiles of 256 x 256; the product alone takes 2.94 ms for
-// 4390 x 128256 x 4096 (1570 TFLOP/s) and 158 us for 6470 x 32000 x 512 (1340: at that depth the epilogue's exponentials, one to 512 multiply-adds, show).
+// 4390 x 128256 x 4096 (1570 TFLOP/s) and 162 us for 6470 x 32000 x 512 (1310: at that depth the epilogue's exponentials, one to 512 multiply-adds, show).
 int tfb::gemm_row_stats(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const int* rows, const int* skip, float2* part, int* status,
                         void* stream) {
   CUtensorMap ta, tb;

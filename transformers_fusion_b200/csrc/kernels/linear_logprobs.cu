@@ -1,4 +1,5 @@
-// Log-probabilities of given tokens under a head, from hidden states: lp = x . w[y] - log sum_v exp(x . w[v]), without the [T, V] logits in memory.
+// Log-probabilities of given tokens under a head, from hidden states: lp = x . w[y] - log sum_v exp(x . w[v]), without the [T, V] logits of many rows in
+// memory.
 //
 //   gather   rows that are scored, one behind the other: a prompt's rows take no part in the product
 //   product  x W^T on tensor cores (gemm_bf16.cu), whose epilogue keeps (m, sum exp) of every row's columns in half a tile, the target's left out, and drops the rest

@@ -456,7 +456,8 @@ class DenseModel(nn.Module):
     @torch.no_grad()
     def score_tokens(self, ids, targets, ignore_index: int = -100):
         """Log-probabilities of given tokens, float32 [B, S]: position s scores targets[b, s] after ids[b, :s + 1]; 0 where the target is ``ignore_index``.
-        For passes that want no gradient: the logits are never in memory, and positions that are not scored take no part in the head's product."""
+        For passes that want no gradient: the [B, S, V] logits are not in memory, and positions that are not scored take no part in the head's product (on the GPU from 65
+        positions on, or 129 at widths of 2048 and more: the logits of fewer, all of them, stand in a float32 workspace)."""
         return linear_logprobs(self.hidden_states(ids).view(*ids.shape, -1), self.lm_head.data, targets, ignore_index)[0]
 
     @torch.no_grad()

@@ -526,7 +526,8 @@ def _tma_ready(t):
 
 
 def linear_logprobs(x, weight, targets, ignore_index: int = -100):
-    """Log-probabilities of given tokens under a head, and the logsumexp of its logits, without all of the logits in memory: x [..., H], weight [V, H] (bfloat16, or
+    """Log-probabilities of given tokens under a head, and the logsumexp of its logits, without the logits of many rows in memory (those of up to 64 rows, or 128 at widths of
+    2048 and more, stand in a float32 workspace on the GPU): x [..., H], weight [V, H] (bfloat16, or
     float32 on the CPU), targets of x's leading shape -> (logp, lse), float32, both 0 where the target is ``ignore_index``.  For passes that want
     no gradient (reference models, older policies, evaluation); with one use ``token_logprobs`` on the logits."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
