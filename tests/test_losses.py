@@ -948,3 +948,43 @@ def test_scoring_of_infinite_logits(dev, M):
         s = z[r, 7].item() if s is None else s
         near(lp[r].cpu(), torch.tensor(l), tol, ("logp", r))
         near(lse[r].cpu(), torch.tensor(s), tol, ("lse", r))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 40, 100])
+def test_scoring_of_few_rows_in_graphs(M):
+    """Two graphs captured on two streams, replayed at once beside eager calls on a third, each with inputs of its own that change between replays."""
+    H, V = 512, 20000
+    x, w, y = exact_products(3 * M, H, V, gen("cuda", M), "cuda")
+    want = L.linear_logprobs(x, w, y)
+    want64 = torch.log_softmax(x.double() @ w.double().t(), -1).gather(1, y.clamp(min=0)[:, None])[:, 0] * (y != IGN)
+    near(want[0], want64, lp_tol(want64))
+    streams, graphs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams[:2]:
+        xs, ys = torch.zeros_like(x[:M]), torch.zeros_like(y[:M])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            L.linear_logprobs(xs, w, ys)
+            s.synchronize()
+            with torch.cuda.graph(graph, stream=s):
+                out = L.linear_logprobs(xs, w, ys)
+        graphs.append((graph, xs, ys, out))
+    torch.cuda.synchronize()
+    for turn in range(4):
+        got = []
+        for i, (s, (graph, xs, ys, out)) in enumerate(zip(streams, graphs)):
+            part = slice((turn + i) % 3 * M, (turn + i) % 3 * M + M)
+            with torch.cuda.stream(s):
+                xs.copy_(x[part])
+                ys.copy_(y[part])
+                graph.replay()
+                got.append((part, [t.clone() for t in out]))
+        with torch.cuda.stream(streams[2]):
+            part = slice((turn + 2) % 3 * M, (turn + 2) % 3 * M + M)
+            got.append((part, L.linear_logprobs(x[part], w, y[part])))
+        torch.cuda.synchronize()
+        for part, (lp, lse) in got:
+            near(lp, want64[part], lp_tol(want64[part]))
+            near(lse, want[1][part], 2 * lp_tol(want[1][part].double()))
+    _lib.check_status()
